@@ -115,7 +115,9 @@ def build_native(force=False):
         hip, _ = _sources()
         obj_dir = os.path.join(CSRC_DIR, '_build')
         os.makedirs(obj_dir, exist_ok=True)
-        flags = ['--offload-arch=' + GPU_ARCH, '-O3', '-std=c++17', '-fPIC', '-Wno-unused-value']
+        # (no packed fp32 instructions: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on gfx950 now and then, and hipcc makes them from ordinary
+        # float code by itself; the host pass does not know the feature and says so)
+        flags = ['--offload-arch=' + GPU_ARCH, '-O3', '-std=c++17', '-fPIC', '-Wno-unused-value', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
 
         def compile_one(src):
             obj = os.path.join(obj_dir, os.path.basename(src)[:-4] + '.o')
