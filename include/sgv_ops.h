@@ -534,6 +534,60 @@ int sgv_multi_nan_to_num_f32(float* const* tensors, const int64_t* numels, int32
 int sgv_multi_scale_f32(const float* const* src, float* const* dst, const int64_t* numels, const float* scales, int32_t count, void* stream);
 
 /* ---------------------------------------------------------------------------------------
+ * Root-mean-square norm of rows (csrc/rms_norm.hip): normalize_2nd_moment (layers.py:16-18) as an operator of its own, with a learned weight per column, the addition
+ * of a residual stream in front of it, and an output in the rows' type or in 8 bits.
+ *   h = T(x + residual)   (h = x without a residual; T: rounding to the rows' type -- the norm sees the h that is written)
+ *   y = h * rsqrt(mean_k h^2 + eps) * weight
+ *   8 bits:  q = 127 h weight / max_k |h weight| rounded to nearest even (exactly: decided in fp64 next to a border), q_scale = max_k |y| / 127;
+ *            a row of zeros has scale 0; a row with a NaN or an infinity in y has scale NaN and zeros
+ * normalize = 0 (8-bit output only): y = h * weight -- the plain quantisation of rows.
+ * Rows are fp32, fp16 or bf16 (`dtype`) with unit stride along a row; x_stride / residual_stride: elements between rows (0: one row for all); y and h are dense.
+ * Rows of q start on 16 bytes; columns from `cols` up to the next multiple of 16 are written with zeros.
+ * inv_rms [rows] (optional): rsqrt(mean h^2 + eps), what the backward pass takes. */
+typedef struct sgv_rms_norm_params {
+    const void* x; const void* residual; const void* weight;
+    void* y; void* h; float* inv_rms;
+    void* q; float* q_scale;                   /* signed bytes; one fp32 scale per row */
+    int64_t rows; int64_t x_stride, residual_stride, q_stride;
+    int32_t cols;
+    int32_t weight_f32;                        /* the weight is fp32 whatever the rows' type */
+    int32_t normalize;
+    float eps;
+} sgv_rms_norm_params;
+int sgv_rms_norm(const sgv_rms_norm_params* p, int dtype, void* stream);
+
+/* With g = dy * weight, xh = h * inv_rms:  dx = inv_rms * (g - xh * mean_k(g xh)) + dh  (the gradient of x and of the residual alike; dh: the gradient that arrives
+ * at h itself, or NULL), dweight = sum over rows of dy * xh (in the weight's type).  dx or dweight may be NULL.  dweight needs a workspace of
+ * sgv_rms_norm_backward_workspace_bytes(); it is written before it is read, and the order of the sum is fixed: equal inputs give equal bits.  dx is dense. */
+typedef struct sgv_rms_norm_backward_params {
+    const void* dy; const void* h; const void* dh; const void* weight; const float* inv_rms;
+    void* dx; void* dweight; void* workspace;
+    int64_t workspace_bytes;
+    int64_t rows; int64_t dy_stride, h_stride, dh_stride;
+    int32_t cols;
+    int32_t weight_f32;
+} sgv_rms_norm_backward_params;
+int64_t sgv_rms_norm_backward_workspace_bytes(int64_t rows, int32_t cols, int dtype);
+int sgv_rms_norm_backward(const sgv_rms_norm_backward_params* p, int dtype, void* stream);
+
+/* out[r, c] = q[r, c] * scale[r], dense rows of `dtype`. */
+int sgv_dequantize_rows(const void* q, int64_t q_stride, const float* scale, void* out, int64_t rows, int32_t cols, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Matrix product in 8-bit integers (csrc/int8_gemm.hip): the dense layer of layers.py:108-138 on quantised rows.
+ *   C[m,n] = act( (sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n] ) * gain       C in `dtype` (fp32, fp16, bf16), sums in 32-bit integers (exact)
+ * Rows of a [m,k] and b [n,k] are signed bytes, start on 16 bytes (base and lda / ldb; rows may overlap, 0: one row for all) and can be READ up to the next multiple of 16 columns: what lies there
+ * is ignored (sgv_rms_norm writes its 8-bit rows that way).  k <= 131071.  bias (fp32) may be NULL. */
+typedef struct sgv_int8_gemm_params {
+    const void* a; const void* b; const float* a_scale; const float* b_scale; const float* bias; void* c;
+    int64_t lda, ldb, ldc;
+    int32_t m, n, k;
+    int32_t act;            /* 1 linear, 3 lrelu */
+    float alpha, gain;
+} sgv_int8_gemm_params;
+int sgv_int8_gemm(const sgv_int8_gemm_params* p, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------
  * Per-launch timing (bench.py roofline leg).  When enabled, every sgv_* launch is bracketed by
  * two HIP events on its own stream; sgv_prof_collect synchronises those events and reports, per
  * kernel family, launch count, summed milliseconds and summed algorithmic bytes
@@ -553,7 +607,9 @@ enum sgv_kernel_family {
     SGV_K_CONV3X3_S1 = 10,      /* conv3x3_ws_kernel (stride 1, forward and data gradient, images >= 32 pixels): the step's dominant kernel */
     SGV_K_FC = 11,              /* sgv_fc (dense layers; the tiled GEMM keeps SGV_K_GEMM) */
     SGV_K_ABSMAX = 12,          /* sgv_absmax: the magnitude-bound passes of the block-scaled fp16 split (timed, not counted by sgv_launch_count) */
-    SGV_K_COUNT = 13
+    SGV_K_RMS_NORM = 13,        /* sgv_rms_norm, its gradient, sgv_dequantize_rows */
+    SGV_K_INT8_GEMM = 14,       /* sgv_int8_gemm */
+    SGV_K_COUNT = 15
 };
 typedef struct sgv_prof_entry {
     int64_t launches;

@@ -184,7 +184,7 @@ def native_loaded():
 c_void_p, c_int, c_int32, c_int64, c_float, c_double = ctypes.c_void_p, ctypes.c_int, ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_double
 
 SGV_F32, SGV_F16, SGV_BF16, SGV_F64 = 0, 1, 2, 3
-SGV_K_NAMES = ['upfirdn2d_rows', 'upfirdn2d_generic', 'bias_act', 'modulate', 'time_encode', 'gemm', 'upfirdn2d_lanes', 'pointwise', 'conv_wrw', 'conv3x3', 'conv3x3_s1', 'fc', 'absmax']
+SGV_K_NAMES = ['upfirdn2d_rows', 'upfirdn2d_generic', 'bias_act', 'modulate', 'time_encode', 'gemm', 'upfirdn2d_lanes', 'pointwise', 'conv_wrw', 'conv3x3', 'conv3x3_s1', 'fc', 'absmax', 'rms_norm', 'int8_gemm']
 
 
 class Upfirdn2dParams(ctypes.Structure):
@@ -264,6 +264,22 @@ class FcParams(ctypes.Structure):
                 ('batch', c_int32), ('a_stride_batch', c_int64), ('b_stride_batch', c_int64), ('c_stride_batch', c_int64), ('accumulate', c_int32)]
 
 
+class RmsNormParams(ctypes.Structure):
+    _fields_ = [('x', c_void_p), ('residual', c_void_p), ('weight', c_void_p), ('y', c_void_p), ('h', c_void_p), ('inv_rms', c_void_p), ('q', c_void_p), ('q_scale', c_void_p),
+                ('rows', c_int64), ('x_stride', c_int64), ('residual_stride', c_int64), ('q_stride', c_int64), ('cols', c_int32), ('weight_f32', c_int32), ('normalize', c_int32),
+                ('eps', c_float)]
+
+
+class RmsNormBackwardParams(ctypes.Structure):
+    _fields_ = [('dy', c_void_p), ('h', c_void_p), ('dh', c_void_p), ('weight', c_void_p), ('inv_rms', c_void_p), ('dx', c_void_p), ('dweight', c_void_p), ('workspace', c_void_p),
+                ('workspace_bytes', c_int64), ('rows', c_int64), ('dy_stride', c_int64), ('h_stride', c_int64), ('dh_stride', c_int64), ('cols', c_int32), ('weight_f32', c_int32)]
+
+
+class Int8GemmParams(ctypes.Structure):
+    _fields_ = [('a', c_void_p), ('b', c_void_p), ('a_scale', c_void_p), ('b_scale', c_void_p), ('bias', c_void_p), ('c', c_void_p),
+                ('lda', c_int64), ('ldb', c_int64), ('ldc', c_int64), ('m', c_int32), ('n', c_int32), ('k', c_int32), ('act', c_int32), ('alpha', c_float), ('gain', c_float)]
+
+
 class ProfRecord(ctypes.Structure):
     _fields_ = [('family', c_int32), ('variant', c_int32), ('ms', c_float), ('reserved', c_float), ('bytes', c_double), ('flops', c_double)]
 
@@ -320,6 +336,11 @@ ABI_SYMBOLS = {
     'sgv_gemm_f32': (c_int, [ctypes.POINTER(GemmParams), c_void_p]),
     'sgv_fc': (c_int, [ctypes.POINTER(FcParams), c_void_p]),
     'sgv_fc_grouped': (c_int, [ctypes.POINTER(FcParams), c_int32, c_void_p]),
+    'sgv_rms_norm': (c_int, [ctypes.POINTER(RmsNormParams), c_int, c_void_p]),
+    'sgv_rms_norm_backward_workspace_bytes': (c_int64, [c_int64, c_int32, c_int]),
+    'sgv_rms_norm_backward': (c_int, [ctypes.POINTER(RmsNormBackwardParams), c_int, c_void_p]),
+    'sgv_dequantize_rows': (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int, c_void_p]),
+    'sgv_int8_gemm': (c_int, [ctypes.POINTER(Int8GemmParams), c_int, c_void_p]),
     'sgv_multi_nan_to_num_f32': (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), c_int32, c_float, c_float, c_float, c_void_p]),
     'sgv_multi_scale_f32': (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), ctypes.POINTER(c_float), c_int32, c_void_p]),
     'sgv_prof_enable': (c_int, [c_int32]),

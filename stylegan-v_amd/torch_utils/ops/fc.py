@@ -214,7 +214,7 @@ def grouped_affine(ws, idx, layers, gains=None):
     gains = [1.0 if g is None else float(g) for g in (gains or [None] * len(layers))]
     ok = (grouped and enabled and ws.is_cuda and ws.ndim == 3 and ws.dtype == torch.float32 and len(layers) > 1 and ws.shape[0] <= 65535 * 32
           and all(l.activation == 'linear' and l.bias is not None and l.weight.dtype == torch.float32 and l.bias.dtype == torch.float32 and l.weight.shape[1] == ws.shape[2]
-                  and l.bias_gain == layers[0].bias_gain for l in layers))
+                  and l.bias_gain == layers[0].bias_gain and not l.serves_int8() for l in layers))
     if not ok:
         return tuple(l(ws[:, i], gain=(None if g == 1.0 else g)) for l, i, g in zip(layers, idx, gains))
     cfg = (tuple(int(i) for i in idx), tuple(float(l.weight_gain) for l in layers), float(layers[0].bias_gain), tuple(gains))

@@ -1,0 +1,121 @@
+"""Dense layers in 8-bit integers (csrc/int8_gemm.hip, csrc/rms_norm.hip): rows quantised with one scale each, and their matrix product.
+
+    quantize_rows(x)                          -> q int8, scale = max|x| / 127 per row
+    matmul(a, a_scale, b, b_scale, ...)       -> act((a b^T) * a_scale * b_scale + bias) * act_gain
+    dense(x, weight, weight_scale, ...)       -> FullyConnectedLayer.forward (src/training/layers.py:108-138) with 8-bit operands
+
+A weight is quantised once (``quantize_rows(weight)``: one scale per output channel), activations at every call (one scale per token).  The sums are exact 32-bit integers,
+so a result depends neither on how the product is split nor on the other rows of a batch; scales, bias and activation are applied in fp32, rounded once to the output's type.
+All of it serves inference and has no gradient.  CPU tensors take the plain torch formulation.
+"""
+import torch
+
+from .. import custom_ops
+from . import bias_act as _ba
+from . import rms_norm as _rn
+
+max_inner = 131071     # 128 * 128 * K has to fit in a signed 32-bit sum
+
+
+def quantize_rows(x):
+    """x [..., K] -> (q [..., K] int8, scale [...] fp32): x stands for q * scale, q = x / scale to nearest even; zero and non-finite rows as in ``rms_norm_int8``.
+    The rows of q start on 16 bytes, as ``matmul`` wants them."""
+    _rn._check('quantize_rows', x, None, None, 0.0)
+    _rn.check_no_grad('quantize_rows', x)
+    if not x.is_cuda:
+        return _rn.quantize_ref(x.double(), 1.0)
+    q, _, _, scale = _rn.launch_forward(_rn.row_view(x), None, None, 0.0, int8=True, normalize=False)
+    if x.ndim != 2:
+        q, scale = q.unflatten(0, x.shape[:-1]) if x.ndim > 2 else q[0], scale.view(x.shape[:-1])
+    return q, scale
+
+
+def dequantize_rows(q, scale, dtype=torch.float32):
+    """q [..., K] int8, scale [...] fp32 -> q * scale in ``dtype``, dense."""
+    _check_rows('dequantize_rows', 'q', q, scale)
+    if dtype not in _rn._DTYPE_CODES:
+        raise RuntimeError(f'dequantize_rows: unsupported dtype {dtype}')
+    _rn.check_no_grad('dequantize_rows', scale)
+    if not q.is_cuda:
+        return (q.float() * scale.unsqueeze(-1)).to(dtype)
+    rows = _rn.row_view(q)
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if rows.shape[0]:
+        lib = custom_ops.get_native()
+        with custom_ops.device_guard(q):
+            custom_ops.check(lib.sgv_dequantize_rows(rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else 0, scale.contiguous().data_ptr(), out.data_ptr(), rows.shape[0], rows.shape[1],
+                                                     _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(q)), lib)
+    return out
+
+
+def _check_rows(what, name, q, scale):
+    if not isinstance(q, torch.Tensor) or q.dtype != torch.int8 or q.ndim < 1 or q.shape[-1] < 1:
+        raise RuntimeError(f'{what}: {name} must be int8 rows (at least one dimension, the last one not empty)')
+    if scale.dtype != torch.float32 or scale.shape != q.shape[:-1] or scale.device != q.device:
+        raise RuntimeError(f'{what}: the scales of {name} must be fp32, one per row, on its device')
+
+
+def _product_rows(q):
+    """(tensor to keep, row stride in bytes): the rows of q starting on 16 bytes and readable up to the next multiple of 16 columns -- q itself where it is so (what
+    ``quantize_rows`` and ``rms_norm_int8`` return, and any dense K % 16 == 0 tensor), else a copy."""
+    q = _rn.row_view(q)
+    rows, cols = q.shape
+    pitch = (cols + 15) // 16 * 16
+    stride = q.stride(0) if rows > 1 else pitch
+    if q.data_ptr() % 16 == 0 and stride % 16 == 0 and (cols == pitch or q.storage_offset() + (rows - 1) * stride + pitch <= q.untyped_storage().nbytes()):
+        return q, stride
+    out = torch.empty([rows, pitch], dtype=torch.int8, device=q.device)
+    out[:, :cols].copy_(q)          # (what lies behind the last column is ignored)
+    return out, pitch
+
+
+def _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype):
+    v = torch.matmul(a.double(), b.double().t()) * a_scale.double().unsqueeze(-1) * b_scale.double()     # (whole numbers below 2^53: exact)
+    if bias is not None:
+        v = v + bias.double()
+    if act == 'lrelu':
+        v = torch.where(v > 0, v, v * _ba.activation_funcs[act].def_alpha)
+    return (v * gain).to(dtype)
+
+
+def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype=torch.float32):
+    """a [..., K] int8 with a_scale [...], b [N, K] int8 with b_scale [N], bias [N] or None -> [..., N] in ``dtype`` (fp32, fp16, bf16).
+    ``act``: 'linear' or 'lrelu'; ``act_gain``: its gain (default: the activation's own, sqrt(2) for lrelu)."""
+    _check_rows('matmul', 'a', a, a_scale)
+    _check_rows('matmul', 'b', b, b_scale)
+    cols = a.shape[-1]
+    if b.ndim != 2 or b.shape[1] != cols or b.device != a.device:
+        raise RuntimeError('matmul: b must be [N, K] with the K of a, on the device of a')
+    if cols > max_inner:
+        raise RuntimeError(f'matmul: K is at most {max_inner} (a sum of 128 * 128 * K has to fit in 32 bits)')
+    if dtype not in _rn._DTYPE_CODES:
+        raise RuntimeError(f'matmul: unsupported dtype {dtype}')
+    if act not in ('linear', 'lrelu'):
+        raise RuntimeError(f'matmul: unsupported activation {act}')
+    if bias is not None and (bias.ndim != 1 or bias.shape[0] != b.shape[0] or bias.dtype != torch.float32 or bias.device != a.device):
+        raise RuntimeError('matmul: bias must be fp32, one element per row of b, on the device of a')
+    _rn.check_no_grad('matmul', a_scale, b_scale, bias)
+    spec = _ba.activation_funcs[act]
+    gain = float(spec.def_gain if act_gain is None else act_gain)
+    if not a.is_cuda:
+        return _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype)
+    n = b.shape[0]
+    out = torch.empty(a.shape[:-1] + (n,), dtype=dtype, device=a.device)
+    if out.numel():
+        ar, lda = _product_rows(a)
+        br, ldb = _product_rows(b)
+        sa, sb = a_scale.contiguous(), b_scale.contiguous()
+        bc = bias.contiguous() if bias is not None else None
+        lib = custom_ops.get_native()
+        p = custom_ops.Int8GemmParams(ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), bc.data_ptr() if bc is not None else None, out.data_ptr(), lda, ldb, n,
+                                      ar.shape[0], n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
+        with custom_ops.device_guard(a):
+            custom_ops.check(lib.sgv_int8_gemm(p, _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(a)), lib)
+    return out
+
+
+def dense(x, weight, weight_scale, bias=None, act='linear', act_gain=None, normalize=False, eps=1e-8):
+    """x [..., K] fp32 / fp16 / bf16, weight [N, K] int8 with weight_scale [N] (``quantize_rows`` of the layer's weight), bias [N] fp32 -> [..., N] in x's type.
+    ``normalize``: the rows of x through ``rms_norm`` (no weight) first, in the same pass that quantises them."""
+    q, scale = _rn.rms_norm_int8(x, eps=eps) if normalize else quantize_rows(x)
+    return matmul(q, scale, weight, weight_scale, bias=bias, act=act, act_gain=act_gain, dtype=x.dtype)

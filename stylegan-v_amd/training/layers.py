@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from ..torch_utils import misc
-from ..torch_utils.ops import bias_act, conv2d_gradfix, conv2d_resample, eqlr, fc, fused_conv_act, fused_down_act, pointwise, upfirdn2d
+from ..torch_utils.ops import bias_act, conv2d_gradfix, conv2d_resample, eqlr, fc, fused_conv_act, fused_down_act, int8, pointwise, upfirdn2d
 
 
 @misc.profiled_function
@@ -34,11 +34,37 @@ class FullyConnectedLayer(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.full([out_features], float(bias_init))) if bias else None
         self.weight_gain = lr_multiplier / math.sqrt(in_features)
         self.bias_gain = lr_multiplier
+        for name in ('weight_int8', 'weight_int8_scale', 'bias_int8'):      # (not in the state dict: derived from the parameters by quantize_int8_)
+            self.register_buffer(name, None, persistent=False)
+        self._int8_of = None
+
+    def _parameter_versions(self):
+        return tuple(None if p is None or p.is_inference() else p._version for p in (self.weight, self.bias))
+
+    def quantize_int8_(self):
+        """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
+        quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters change
+        afterwards (an optimiser step, ``load_state_dict``) refuses to serve until it is quantised again.  Returns the layer."""
+        if self.activation not in ('linear', 'lrelu'):
+            raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
+        with torch.no_grad():
+            self.weight_int8, self.weight_int8_scale = int8.quantize_rows(self.weight.float() * self.weight_gain)
+            self.bias_int8 = self.bias.float() * self.bias_gain if self.bias is not None else None
+        self._int8_of = self._parameter_versions()
+        return self
+
+    def serves_int8(self):
+        return self.weight_int8 is not None and not torch.is_grad_enabled()
 
     def forward(self, x, normalize_input=False, gain=None):
         """``normalize_input``: apply normalize_2nd_moment to x first (the mapping network's first layer; one kernel with the layer).
         ``gain``: the layer's output times a constant (ToRGB's ``affine(w) * weight_gain``, networks.py:314) -- rides on the kernel's activation gain instead of
         costing a launch here and another in the backward pass."""
+        if self.serves_int8():
+            if self._parameter_versions() != self._int8_of:
+                raise RuntimeError('the parameters of this layer changed after quantize_int8_(): quantise it again')
+            act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
+            return int8.dense(x, self.weight_int8, self.weight_int8_scale, self.bias_int8, act=self.activation, act_gain=act_gain, normalize=normalize_input)
         if x.ndim == 2:   # one kernel on the GPU (ops/fc.py -> csrc/fc.hip); the torch composition elsewhere
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
             return fc.dense(x, self.weight, self.bias, weight_gain=self.weight_gain, bias_gain=self.bias_gain, act=self.activation, normalize=normalize_input, act_gain=act_gain)
@@ -79,6 +105,14 @@ class MappingNetwork(torch.nn.Module):
             setattr(self, f'fc{idx}', FullyConnectedLayer(fin, fout, activation=activation, lr_multiplier=lr_multiplier))
         if num_ws is not None and w_avg_beta is not None:
             self.register_buffer('w_avg', torch.zeros([w_dim]))
+
+    def quantize_int8_(self):
+        """Serve the network's dense layers in 8-bit integers (``FullyConnectedLayer.quantize_int8_``): under ``torch.no_grad()`` an unconditional network is one norm +
+        quantisation, one product per layer and one quantisation between two layers.  For a generator that serves: ``G_ema.mapping.quantize_int8_()``."""
+        for module in self.modules():
+            if isinstance(module, FullyConnectedLayer):
+                module.quantize_int8_()
+        return self
 
     def forward(self, z, c, truncation_psi=1, truncation_cutoff=None, skip_w_avg_update=False):
         parts = []

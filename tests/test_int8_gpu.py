@@ -1,0 +1,199 @@
+"""8-bit product (csrc/int8_gemm.hip through ops/int8.py) against 64-bit arithmetic, and the operators together as they are served.
+
+The sums are whole numbers and exact.  The epilogue in fp32 (U = 2^-24): one rounding each for the sum as a float, times a_scale, times b_scale plus bias, times the
+slope and the gain (both constants rounded too): 3 U of |sum * scales| and 5 U of the result, then half a step of the output's type."""
+import pytest
+import torch
+
+from stylegan_v_amd.torch_utils import custom_ops
+from stylegan_v_amd.torch_utils.ops import int8, rms_norm as rn
+from stylegan_v_amd.training.layers import FullyConnectedLayer, MappingNetwork
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+U = 2.0 ** -24
+
+
+def _bytes(m, k, seed):
+    return torch.randint(-128, 128, [m, k], generator=torch.Generator(device=DEV).manual_seed(seed), dtype=torch.int8, device=DEV)
+
+
+def _scales(n, seed):
+    return torch.rand([n], generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV) * 0.02 + 0.001
+
+
+def _sums(a, b):
+    if a.numel() * b.shape[0] > 1 << 33:
+        return torch.matmul(a.double(), b.double().t().contiguous())
+    return torch.matmul(a.double().cpu(), b.double().cpu().t()).to(a.device)
+
+
+def _verify(got, a, sa, b, sb, bias, act, gain, dtype):
+    prod = _sums(a, b) * sa.double().unsqueeze(1) * sb.double()
+    v = prod if bias is None else prod + bias.double()
+    if act == 'lrelu':
+        v = torch.where(v > 0, v, v * 0.2)
+    v = v * gain
+    tol = 3 * U * prod.abs() * gain + 5 * U * v.abs() + torch.finfo(dtype).eps / 2 * v.abs() * 1.0001 + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    assert got.dtype == dtype and got.shape == v.shape
+    err = (got.double() - v).abs()
+    assert (err <= tol).all(), f'{(err / tol).max().item():.3g} of the tolerance, first at {(err > tol).nonzero()[0].tolist()}'
+
+
+SIZES = [(1, 1, 1), (1, 512, 512), (1, 1000, 8192), (2, 17, 16), (7, 33, 15), (15, 16, 64), (16, 16, 65), (17, 64, 63), (32, 512, 8192), (33, 31, 129), (64, 100, 1000), (65, 130, 17),
+         (100, 513, 48), (127, 128, 128), (128, 127, 2047), (129, 257, 2048), (200, 300, 2049), (255, 256, 100), (256, 255, 4096), (257, 300, 333), (511, 1025, 1030), (513, 512, 512),
+         (1000, 1001, 1003), (1025, 520, 144), (2049, 1000, 272), (3000, 2100, 640)]
+
+
+@pytest.mark.parametrize('m,n,k', SIZES)
+def test_product(m, n, k):
+    g = torch.Generator(device=DEV).manual_seed(m * n + k)
+    a, b, sa, sb = _bytes(m, k, m + 1), _bytes(n, k, n + 2), _scales(m, 3), _scales(n, 4)
+    bias = torch.randn([n], generator=g, device=DEV)
+    before = custom_ops.launch_count()
+    got = int8.matmul(a, sa, b, sb)
+    assert custom_ops.launch_count() - before == 1
+    _verify(got, a, sa, b, sb, None, 'linear', 1.0, torch.float32)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        _verify(int8.matmul(a, sa, b, sb, bias=bias, act='lrelu', dtype=dtype), a, sa, b, sb, bias, 'lrelu', 2 ** 0.5, dtype)
+    _verify(int8.matmul(a, sa, b, sb, bias=bias, act_gain=0.5), a, sa, b, sb, bias, 'linear', 0.5, torch.float32)
+
+
+@pytest.mark.parametrize('m,n', [(1, 40), (3, 8), (40, 70), (300, 520), (600, 300)])
+def test_extreme_bytes_and_longest_sums(m, n):
+    """-128 times -128 over the longest K that 32 bits hold, and bytes behind the last column that must not count."""
+    k = int8.max_inner
+    a, b = torch.full([m, k], -128, dtype=torch.int8, device=DEV), torch.full([n, k], -128, dtype=torch.int8, device=DEV)
+    one_m, one_n = torch.ones(m, device=DEV), torch.ones(n, device=DEV)
+    assert torch.equal(int8.matmul(a, one_m, b, one_n), torch.full([m, n], float(128 * 128 * k), device=DEV))
+    for k in (1, 5, 16, 17, 31, 33, 64, 100, 127, 129, 200, 255, 257):
+        wide_a, wide_b = torch.full([m, 272], 127, dtype=torch.int8, device=DEV), torch.full([n, 272], 127, dtype=torch.int8, device=DEV)
+        a, b = wide_a[:, :k], wide_b[:, :k]
+        a.fill_(1)
+        b.fill_(-1)
+        assert torch.equal(int8.matmul(a, one_m, b, one_n), torch.full([m, n], -float(k), device=DEV))
+
+
+def test_strides_alignments_and_shapes():
+    base, wb = _bytes(70, 400, 1), _bytes(90, 400, 2)
+    for cut in (lambda t: t[:, 16:336], lambda t: t[:, 1:300], lambda t: t[:, :39], lambda t: t[::2, 32:], lambda t: t[:, ::2], lambda t: t[5:6], lambda t: t[1:2].expand(40, 400),
+                lambda t: t[:64].t(), lambda t: t[-3:, -33:], lambda t: t.as_strided([20, 48], [16, 1])):
+        a, b = cut(base), cut(wb)
+        sa, sb = _scales(a.shape[0], 1), _scales(b.shape[0], 2)
+        _verify(int8.matmul(a, sa, b, sb), a, sa, b, sb, None, 'linear', 1.0, torch.float32)
+    a, sa, sb = base.view(7, 10, 400), _scales(70, 1).view(7, 10), _scales(90, 2)
+    got = int8.matmul(a, sa, wb, sb)
+    assert got.shape == (7, 10, 90) and torch.equal(got.view(70, 90), int8.matmul(base, sa.view(70), wb, sb))
+    assert torch.equal(int8.matmul(base[3], sa.view(70)[3], wb, sb), got.view(70, 90)[3])
+    assert int8.matmul(base[:0], sa.view(70)[:0], wb, sb).shape == (0, 90) and int8.matmul(base, sa.view(70), wb[:0], sb[:0]).shape == (70, 0)
+    sliced = int8.matmul(base, _scales(140, 1)[::2], wb, _scales(180, 2)[::2])          # scales with strides
+    assert torch.equal(sliced, int8.matmul(base, _scales(140, 1)[::2].contiguous(), wb, _scales(180, 2)[::2].contiguous()))
+
+
+def test_a_row_does_not_depend_on_its_batch():
+    a, b, sa, sb = _bytes(700, 1000, 1), _bytes(600, 1000, 2), _scales(700, 3), _scales(600, 4)
+    full = int8.matmul(a, sa, b, sb)
+    for m in (1, 16, 17, 40, 100, 257, 513):
+        assert torch.equal(int8.matmul(a[:m], sa[:m], b, sb), full[:m])
+
+
+def test_scales_that_are_not_numbers():
+    a, b, sa, sb = _bytes(40, 64, 1), _bytes(50, 64, 2), _scales(40, 3), _scales(50, 4)
+    a[4] = 0
+    sa[4], sb[7], sa[9] = float('nan'), float('inf'), 0.0
+    got = int8.matmul(a, sa, b, sb)
+    assert got[4].isnan().all()
+    keep = torch.ones(40, dtype=torch.bool, device=DEV)
+    keep[4] = False
+    assert not torch.isfinite(got[keep][:, 7]).any() and torch.isfinite(got[keep][:, :7]).all() and not got[9, :7].any()
+
+
+def test_refusals_on_the_gpu():
+    a, b, sa, sb = _bytes(4, 64, 1), _bytes(5, 64, 2), _scales(4, 3), _scales(5, 4)
+    for bad in ((a.cpu(), sa, b, sb), (a, sa.cpu(), b, sb), (a, sa, b.cpu(), sb), (a, sa, b, sb.cpu())):
+        with pytest.raises(RuntimeError, match='device'):
+            int8.matmul(*bad)
+    with pytest.raises(RuntimeError, match='device'):
+        int8.matmul(a, sa, b, sb, bias=torch.zeros(5))
+
+
+def test_dense_is_quantise_and_product():
+    x = torch.randn([77, 333], generator=torch.Generator().manual_seed(0)).to(DEV)
+    w, bias = torch.randn([50, 333], generator=torch.Generator().manual_seed(1)).to(DEV), torch.randn([50], device=DEV)
+    wq, ws = int8.quantize_rows(w)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        xt = x.to(dtype)
+        for normalize in (False, True):
+            before = custom_ops.launch_count()
+            got = int8.dense(xt, wq, ws, bias=bias, act='lrelu', normalize=normalize)
+            assert custom_ops.launch_count() - before == 2
+            q, s = rn.rms_norm_int8(xt) if normalize else int8.quantize_rows(xt)
+            assert torch.equal(got, int8.matmul(q, s, wq, ws, bias=bias, act='lrelu', dtype=dtype))
+            _verify(got, q, s, wq, ws, bias, 'lrelu', 2 ** 0.5, dtype)
+
+
+@pytest.mark.parametrize('batch', [1, 32, 1000])
+def test_mapping_network_served_in_8_bits(batch):
+    """The operators together, as the generator's mapping network is served: the same numbers as the CPU formulation of the layers, and near the fp32 network."""
+    torch.manual_seed(0)
+    net = MappingNetwork(z_dim=512, c_dim=0, w_dim=512, num_ws=14, num_layers=2).to(DEV).eval()
+    z, c = torch.randn([batch, 512], device=DEV), torch.zeros([batch, 0], device=DEV)
+    with torch.no_grad():
+        want = net(z, c)
+        net.quantize_int8_()
+        before = custom_ops.launch_count()
+        got = net(z, c)
+        assert custom_ops.launch_count() - before == 4
+        x = z.cpu()
+        for i in range(2):
+            fc = getattr(net, f'fc{i}')
+            x = int8.dense(x, fc.weight_int8.cpu(), fc.weight_int8_scale.cpu(), fc.bias_int8.cpu(), act='lrelu', normalize=(i == 0))
+    # the fp32 sums between the layers differ by a few U, which moves a value across a border of its 8-bit grid now and then: one step, 1/127 of a row's largest value,
+    # in one of its 512 columns; the whole result stays within a hundredth of that
+    assert (got[:, 0].cpu() - x).norm() / x.norm() < 1e-3
+    assert (got - want).norm() / want.norm() < 0.03      # two layers, two operands each: 2 * (3.5 / 127 / sqrt(12)) * sqrt(2) = 2.2 %
+    ref = net.train()(z, c, skip_w_avg_update=True)      # gradients enabled: the fp32 layers
+    # (csrc/fc.hip adds a row's squares from up to 16 waves in any order: 16 U in the sum, 8 U = 5e-7 in the normalised row, about as much in the result)
+    assert ref.requires_grad and (ref.detach() - want).norm() / want.norm() < 1e-5
+
+
+def test_streams_and_graph_replays():
+    torch.manual_seed(0)
+    layer = FullyConnectedLayer(300, 200, activation='lrelu').to(DEV).quantize_int8_()
+    x = torch.randn([500, 300], device=DEV)
+    with torch.no_grad():
+        want = layer(x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = layer(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(got, want)
+        graphs, outs = [], []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                outs.append(layer(x))
+            graphs.append(g)
+        for seed in range(3):
+            x.copy_(torch.randn([500, 300], generator=torch.Generator().manual_seed(seed)))
+            for g in graphs:
+                g.replay()
+            torch.cuda.synchronize()
+            want = layer(x)
+            assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+def test_offsets_beyond_2_31_bytes():
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip('needs 40 GB of device memory')
+    m, k, n = 270000, 8192, 40
+    a = torch.empty([m, k], dtype=torch.int8, device=DEV)
+    a.random_(-128, 128, generator=torch.Generator(device=DEV).manual_seed(0))
+    b, sa, sb = _bytes(n, k, 1), _scales(m, 2), _scales(n, 3)
+    pick = torch.tensor([0, 1, m // 2, 262143, 262144, 262145, m - 1], device=DEV)
+    got = int8.matmul(a, sa, b, sb)
+    _verify(got[pick], a[pick], sa[pick], b, sb, None, 'linear', 1.0, torch.float32)
+    # ... and as the right operand, with a long output row
+    got = int8.matmul(b, sb, a, sa)
+    _verify(got[:, pick], b, sb, a[pick], sa[pick], None, 'linear', 1.0, torch.float32)
