@@ -107,8 +107,11 @@ def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype
         sa, sb = a_scale.contiguous(), b_scale.contiguous()
         bc = bias.contiguous() if bias is not None else None
         lib = custom_ops.get_native()
-        p = custom_ops.Int8GemmParams(ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), bc.data_ptr() if bc is not None else None, out.data_ptr(), lda, ldb, n,
-                                      ar.shape[0], n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
+        m = ar.shape[0]
+        size = lib.sgv_int8_gemm_workspace_bytes(m, n, cols, lda, ldb)
+        work = torch.empty([size], dtype=torch.uint8, device=a.device) if size else None
+        p = custom_ops.Int8GemmParams(ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), bc.data_ptr() if bc is not None else None, out.data_ptr(),
+                                      work.data_ptr() if size else None, size, lda, ldb, n, m, n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
         with custom_ops.device_guard(a):
             custom_ops.check(lib.sgv_int8_gemm(p, _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(a)), lib)
     return out

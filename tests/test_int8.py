@@ -105,4 +105,4 @@ def test_argument_checks_of_the_c_entry_without_gpu():
     assert lib.sgv_int8_gemm(p, custom_ops.SGV_F64, None) == -3
     p.m = 0
     assert lib.sgv_int8_gemm(p, F32, None) == 0
-    assert ctypes.sizeof(custom_ops.Int8GemmParams) == 96
+    assert ctypes.sizeof(custom_ops.Int8GemmParams) == 112
