@@ -577,17 +577,14 @@ int sgv_dequantize_rows(const void* q, int64_t q_stride, const float* scale, voi
  * Matrix product in 8-bit integers (csrc/int8_gemm.hip): the dense layer of layers.py:108-138 on quantised rows.
  *   C[m,n] = act( (sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n] ) * gain       C in `dtype` (fp32, fp16, bf16), sums in 32-bit integers (exact)
  * Rows of a [m,k] and b [n,k] are signed bytes, start on 16 bytes (base and lda / ldb; rows may overlap, 0: one row for all) and can be READ up to the next multiple of 16 columns: what lies there
- * is ignored (sgv_rms_norm writes its 8-bit rows that way).  k <= 131071.  bias (fp32) may be NULL.  Sizes for which sgv_int8_gemm_workspace_bytes() is not 0
- * (few tiles, a long k) need that much workspace on 16 bytes; it is written before it is read. */
+ * is ignored (sgv_rms_norm writes its 8-bit rows that way).  k <= 131071.  bias (fp32) may be NULL.  Rows are at most 8 MB apart. */
 typedef struct sgv_int8_gemm_params {
-    const void* a; const void* b; const float* a_scale; const float* b_scale; const float* bias; void* c; void* workspace;
-    int64_t workspace_bytes;
+    const void* a; const void* b; const float* a_scale; const float* b_scale; const float* bias; void* c;
     int64_t lda, ldb, ldc;
     int32_t m, n, k;
     int32_t act;            /* 1 linear, 3 lrelu */
     float alpha, gain;
 } sgv_int8_gemm_params;
-int64_t sgv_int8_gemm_workspace_bytes(int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb);
 int sgv_int8_gemm(const sgv_int8_gemm_params* p, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------------------

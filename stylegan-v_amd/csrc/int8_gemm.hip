@@ -6,10 +6,6 @@
 // (row = lane & 15, bytes 16 (lane >> 4) ..+15 of 64).  The integer sums are exact whatever their order, so K is split freely -- over the waves of a workgroup, over
 // workgroups -- and the result depends neither on the split nor on the other rows of a batch.
 //
-// Three forms, chosen in sgv_int8_gemm by how many workgroups they make and what each has to read:
-//   int8_rows_kernel   few rows: bound by reading B once
-//   int8_tile_kernel   tiles of C through LDS: bound by the matrix pipe (large) or by the latency of a tile's K loop (few tiles)
-//   ... with K split over workgroups into 32-bit partial tiles, and int8_sum_kernel behind it
 #include "sgv_common.h"
 
 #include <algorithm>
@@ -28,7 +24,6 @@ struct args {
     int lrelu;
     float alpha, gain;
     int tiles_m, tiles_n;
-    int slice;               // k per workgroup (a multiple of 128; the whole of k: no split); slice z writes its sums at c + z * m * ldc
 };
 
 // 16 bytes of a row, `left` of them in front of K: the others are cleared (in one operand: 0 times anything is 0)
@@ -49,63 +44,6 @@ __device__ __forceinline__ float finish(const args& p, int acc, float sa, float 
 }
 
 // ---------------------------------------------------------------------------------------------------------------------------------------
-// Few rows: a workgroup owns 16 MT rows x 16 columns, its waves split K, the partial sums meet in LDS.  Operands go from memory to registers: B is used MT times per
-// wave, there is nothing to share.  U steps of 64 k are loaded together.
-template <typename T, int MT, int U>
-__global__ __launch_bounds__(1024) void int8_rows_kernel(const args p) {
-    extern __shared__ int red[];                 // [waves][MT * 256]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * MT);
-    const int r = lane & 15, kq = (lane >> 4) * 16;
-    const int8_t* b = p.b + (int64_t)min(n0 + r, p.n - 1) * p.ldb + kq;
-    const int8_t* a[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) a[t] = p.a + (int64_t)min(m0 + 16 * t + r, p.m - 1) * p.lda + kq;
-    i32x4 acc[MT];
-#pragma unroll
-    for (int t = 0; t < MT; t++) acc[t] = i32x4{0, 0, 0, 0};
-    const int steps = (p.k + 63) / 64, per = (steps + waves - 1) / waves;
-    const int first = min(wave * per, steps), last = min(first + per, steps);           // a wave's steps are consecutive: whole cache lines
-    int s = first;
-    for (; s + U <= last && (s + U) * 64 <= p.k; s += U) {
-        i32x4 av[U][MT], bv[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            bv[u] = *(const i32x4*)(b + (s + u) * 64);
-#pragma unroll
-            for (int t = 0; t < MT; t++) av[u][t] = *(const i32x4*)(a[t] + (s + u) * 64);
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int t = 0; t < MT; t++) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[u][t], bv[u], acc[t], 0, 0, 0);
-    }
-    for (; s < last; s++) {
-        const int left = p.k - s * 64 - kq;
-        const bool ok = left > 0;
-        const i32x4 bv = mask_tail(ok ? *(const i32x4*)(b + s * 64) : i32x4{0, 0, 0, 0}, left);
-#pragma unroll
-        for (int t = 0; t < MT; t++) {
-            const i32x4 av = ok ? *(const i32x4*)(a[t] + s * 64) : i32x4{0, 0, 0, 0};
-            acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av, bv, acc[t], 0, 0, 0);
-        }
-    }
-    // C layout of the instruction: column = lane & 15, row = 4 * (lane >> 4) + e
-#pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) red[wave * (MT * 256) + t * 256 + ((lane >> 4) * 4 + e) * 16 + r] = acc[t][e];
-    __syncthreads();
-    for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
-        const int m = m0 + (i >> 4), n = n0 + (i & 15);
-        if (m >= p.m || n >= p.n) continue;
-        int sum = red[i];
-        for (int w = 1; w < waves; w++) sum += red[w * (MT * 256) + i];
-        sgv_traits<T>::store((T*)p.c + (int64_t)m * p.ldc + n, finish(p, sum, p.a_scale[m], p.b_scale[n], p.bias ? p.bias[n] : 0.f));
-    }
-}
-
-// ---------------------------------------------------------------------------------------------------------------------------------------
 // Tiles of C.  K is walked in stages of 128 bytes per row -- a cache line -- that go from memory straight into LDS (buffer_load ... lds: no registers, no instructions
 // to store them), S stages in a ring.  A stage's 16-byte chunks lie at position chunk ^ ((row >> 1) & 7) of their row, which makes the fragment reads below free of
 // bank conflicts.  A wave holds the fragments of one step of 64 k in registers and replaces each as soon as its last product is issued, so that the matrix pipe finds
@@ -121,12 +59,92 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff, i
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" :: "s"(lds), "v"(voff), "s"(rsrc), "s"(soff) : "memory");
 }
 
+// ---------------------------------------------------------------------------------------------------------------------------------------
+// Few tiles: every wave of a workgroup computes the whole 16 MT x 16 NT tile over its own stages of K (128 bytes per row; wave w takes stages w, w + waves, ...), in a
+// ring of S stages of LDS of its own -- no barrier in the loop --, and the waves' sums meet in LDS.  Through LDS because the matrix instruction wants 16 rows side by side:
+// read straight into registers, 16 neighbouring lanes touch 16 cache lines, and a CU gets 16 bytes a clock instead of 64 (32 x 512 x 8192: 13.0 us).
+template <typename T, int MT, int NT, int S>
+__global__ __launch_bounds__(512) void int8_rows_kernel(const args p) {
+    extern __shared__ __attribute__((aligned(128))) int8_t ring[];          // [waves][S][(MT + NT) * 16 rows][128], then [waves][MT * NT * 256] sums
+    constexpr int STAGE = (MT + NT) * 2048, LPS = 2 * (MT + NT);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT), k16 = (p.k + 15) & ~15;
+    const int quarter = lane >> 4, r = lane & 15;
+    const i32x4 ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(p.m - 1 - m0) * p.lda + k16);
+    const i32x4 rb = make_rsrc(p.b + (int64_t)n0 * p.ldb, (int64_t)(p.n - 1 - n0) * p.ldb + k16);
+    const i32x4 none = make_rsrc(p.a, 0);
+    unsigned va[2 * MT], vb[2 * NT];
+#pragma unroll
+    for (int i = 0; i < 2 * MT; i++) { const int row = i * 8 + (lane >> 3); va[i] = row * (unsigned)p.lda + ((lane & 7) ^ ((row >> 1) & 7)) * 16; }
+#pragma unroll
+    for (int i = 0; i < 2 * NT; i++) { const int row = i * 8 + (lane >> 3); vb[i] = row * (unsigned)p.ldb + ((lane & 7) ^ ((row >> 1) & 7)) * 16; }
+    const int nst = (p.k + 127) / 128;
+    int8_t* mine = ring + wave * S * STAGE;
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) int8_t*)mine;
+    auto issue = [&](int t, int slot) {
+        const unsigned s = lds0 + slot * STAGE;
+        const int k0 = t < nst ? t * 128 : 0;
+        const i32x4 xa = t < nst ? ra : none, xb = t < nst ? rb : none;
+#pragma unroll
+        for (int i = 0; i < 2 * NT; i++) dma16(xb, s + i * 1024, vb[i], k0);
+#pragma unroll
+        for (int i = 0; i < 2 * MT; i++) dma16(xa, s + NT * 2048 + i * 1024, va[i], k0);
+    };
+    i32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < S; u++) issue(wave + u * waves, u);
+    const int base = r * 128, c0 = (quarter ^ ((r >> 1) & 7)) * 16, c1 = ((4 + quarter) ^ ((r >> 1) & 7)) * 16;
+    int slot = 0;
+    for (int t = wave; t < nst; t += waves) {
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * LPS) : "memory");
+        const int8_t* s = mine + slot * STAGE + base;
+        i32x4 f[2][MT + NT];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < MT + NT; i++) f[h][i] = *(const i32x4*)(s + i * 2048 + (h ? c1 : c0));
+        const int left = p.k - t * 128;
+        if (left < 128) {
+#pragma unroll
+            for (int j = 0; j < NT; j++) { f[0][j] = mask_tail(f[0][j], left - quarter * 16); f[1][j] = mask_tail(f[1][j], left - 64 - quarter * 16); }
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                // (the stage is in registers: its slot may be written over)
+        issue(t + S * waves, slot);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[h][NT + i], f[h][j], acc[i][j], 0, 0, 0);
+        slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+    // D layout of the instruction: column = lane & 15, row = 4 * (lane >> 4) + e
+    int* red = (int*)ring;
+    constexpr int TILE = MT * NT * 256;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) red[wave * TILE + (i * 16 + quarter * 4 + e) * (NT * 16) + j * 16 + r] = acc[i][j][e];
+    __syncthreads();
+    for (int x = threadIdx.x; x < TILE; x += blockDim.x) {
+        const int m = m0 + x / (NT * 16), n = n0 + x % (NT * 16);
+        if (m >= p.m || n >= p.n) continue;
+        int sum = red[x];
+        for (int w = 1; w < waves; w++) sum += red[w * TILE + x];
+        sgv_traits<T>::store((T*)p.c + (int64_t)m * p.ldc + n, finish(p, sum, p.a_scale[m], p.b_scale[n], p.bias ? p.bias[n] : 0.f));
+    }
+}
+
 // four consecutive columns as they are stored
 template <typename T> struct quad;
-template <> struct quad<int> {
-    typedef i32x4 type;
-    static __device__ __forceinline__ type make(const args&, const i32x4& acc, float, const f32x4&, const f32x4&) { return acc; }
-};
 __device__ __forceinline__ f32x4 finish4(const args& p, const i32x4& acc, float sa, const f32x4& sb, const f32x4& bias) {
     return f32x4{finish(p, acc[0], sa, sb[0], bias[0]), finish(p, acc[1], sa, sb[1], bias[1]), finish(p, acc[2], sa, sb[2], bias[2]), finish(p, acc[3], sa, sb[3], bias[3])};
 }
@@ -154,7 +172,6 @@ template <typename T, int BM, int BN, int WGM, int WGN, int S, int LEAD>
 __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p) {
     constexpr int BK = 128, CPR = BK / 16, RPI = 64 / CPR;                // chunks per row, rows per DMA instruction
     constexpr int WAVES = WGM * WGN, TM = BM / WGM / 16, TN = BN / WGN / 16, STAGE = (BM + BN) * BK, LA = BM / RPI / WAVES, LB = BN / RPI / WAVES, LPS = LA + LB;
-    constexpr bool PARTIAL = sizeof(T) == 4 && __is_same(T, int);
     __shared__ __attribute__((aligned(128))) int8_t lds[S * STAGE];
     __shared__ __attribute__((aligned(16))) float sb_lds[BN], bias_lds[BN];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -166,9 +183,9 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
     }
     const int per = 8 * p.tiles_n, first = id / per * 8, rows8 = min(p.tiles_m - first, 8);
     const int m0 = (first + (id % per) % rows8) * BM, n0 = ((id % per) / rows8) * BN;
-    const int kbase = blockIdx.y * p.slice, k = min(p.k - kbase, p.slice), k16 = (k + 15) & ~15;
-    const i32x4 ra = make_rsrc(p.a + (int64_t)m0 * p.lda + kbase, (int64_t)(p.m - 1 - m0) * p.lda + k16);
-    const i32x4 rb = make_rsrc(p.b + (int64_t)n0 * p.ldb + kbase, (int64_t)(p.n - 1 - n0) * p.ldb + k16);
+    const int k = p.k, k16 = (k + 15) & ~15;
+    const i32x4 ra = make_rsrc(p.a + (int64_t)m0 * p.lda, (int64_t)(p.m - 1 - m0) * p.lda + k16);
+    const i32x4 rb = make_rsrc(p.b + (int64_t)n0 * p.ldb, (int64_t)(p.n - 1 - n0) * p.ldb + k16);
     const i32x4 none = make_rsrc(p.a, 0);                                // (stages behind the last one: nothing is fetched, and the count of loads stays the same)
     unsigned va[LA], vb[LB];
     auto swizzle = [](int row) { return (row >> 1) & 7; };
@@ -192,16 +209,14 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
     // the scales of the tile: in flight beside the first stages
     constexpr int PER = (BN + 64 * WAVES - 1) / (64 * WAVES);
     float sa[TM], sbv[PER], biv[PER];
-    if constexpr (!PARTIAL) {
 #pragma unroll
-        for (int i = 0; i < TM; i++) { const int m = m0 + (wm * TM + i) * 16 + r; sa[i] = m < p.m ? p.a_scale[m] : 0.f; }
+    for (int i = 0; i < TM; i++) { const int m = m0 + (wm * TM + i) * 16 + r; sa[i] = m < p.m ? p.a_scale[m] : 0.f; }
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int x = i * 64 * WAVES + threadIdx.x, n = n0 + x;
-            const bool ok = x < BN && n < p.n;
-            sbv[i] = ok ? p.b_scale[n] : 0.f;
-            biv[i] = ok && p.bias ? p.bias[n] : 0.f;
-        }
+    for (int i = 0; i < PER; i++) {
+        const int x = i * 64 * WAVES + threadIdx.x, n = n0 + x;
+        const bool ok = x < BN && n < p.n;
+        sbv[i] = ok ? p.b_scale[n] : 0.f;
+        biv[i] = ok && p.bias ? p.bias[n] : 0.f;
     }
     i32x4 acc[TM][TN];
 #pragma unroll
@@ -270,115 +285,91 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
     // Strips of 16 rows go through a wave's own piece of LDS, so that rows of C leave in 16-byte pieces.
     constexpr int ES = sizeof(T), PITCH = TN * 16 * ES + 16, CH = TN * ES, PCS = 16 / ES;
     static_assert(WAVES * 16 * PITCH <= S * STAGE && (16 * CH) % 64 == 0, "");
-    if constexpr (!PARTIAL) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) { const int x = i * 64 * WAVES + threadIdx.x; if (x < BN) { sb_lds[x] = sbv[i]; bias_lds[x] = biv[i]; } }
-    }
+    for (int i = 0; i < PER; i++) { const int x = i * 64 * WAVES + threadIdx.x; if (x < BN) { sb_lds[x] = sbv[i]; bias_lds[x] = biv[i]; } }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");            // (every load into LDS has landed, the empty ones too: the ring may be written over)
     __builtin_amdgcn_s_barrier();
     int8_t* buf = lds + wave * 16 * PITCH;
-    const int nb = n0 + wn * TN * 16, ncols = PARTIAL ? (int)p.ldc : p.n;
-    const bool whole = m0 + BM <= p.m && n0 + BN <= ncols;
-    T* out = (T*)p.c + (PARTIAL ? (int64_t)blockIdx.y * p.m * p.ldc : 0);
+    const int nb = n0 + wn * TN * 16;
+    const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;
 #pragma unroll
     for (int i = 0; i < TM; i++) {
 #pragma unroll
         for (int j = 0; j < TN; j++) {
             const int x = j * 16 + 4 * quarter;
-            f32x4 s4 = {0.f, 0.f, 0.f, 0.f}, b4 = {0.f, 0.f, 0.f, 0.f};
-            if constexpr (!PARTIAL) { s4 = *(const f32x4*)(sb_lds + wn * TN * 16 + x); b4 = *(const f32x4*)(bias_lds + wn * TN * 16 + x); }
-            *(typename quad<T>::type*)(buf + r * PITCH + x * ES) = quad<T>::make(p, acc[i][j], PARTIAL ? 0.f : sa[i], s4, b4);
+            const f32x4 s4 = *(const f32x4*)(sb_lds + wn * TN * 16 + x), b4 = *(const f32x4*)(bias_lds + wn * TN * 16 + x);
+            *(typename quad<T>::type*)(buf + r * PITCH + x * ES) = quad<T>::make(p, acc[i][j], sa[i], s4, b4);
         }
         const int mb = m0 + (wm * TM + i) * 16;
 #pragma unroll
         for (int q = 0; q < 16 * CH / 64; q++) {
             const int idx = q * 64 + lane, rr = idx / CH, ch = idx % CH, n = nb + ch * PCS;
-            T* o = out + (int64_t)(mb + rr) * p.ldc + n;
+            T* o = (T*)p.c + (int64_t)(mb + rr) * p.ldc + n;
             const i32x4 v = *(const i32x4*)(buf + rr * PITCH + ch * 16);
-            if (whole || (mb + rr < p.m && n + PCS <= ncols)) ((any_i32x4*)o)->v = v;
+            if (whole || (mb + rr < p.m && n + PCS <= p.n)) ((any_i32x4*)o)->v = v;
             else if (mb + rr < p.m)
-                for (int x = 0; n + x < ncols; x++) o[x] = ((const T*)(buf + rr * PITCH + ch * 16))[x];
+                for (int x = 0; n + x < p.n; x++) o[x] = ((const T*)(buf + rr * PITCH + ch * 16))[x];
         }
     }
 }
 
-// C from the partial sums [slices][m][ldp] of a product whose K was split; ldp is a multiple of 4, a thread takes four columns
-template <typename T>
-__global__ __launch_bounds__(256) void int8_sum_kernel(const args p, const int* part, int64_t ldp, int slices) {
-    const int64_t quads = ldp / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= quads * p.m) return;
-    const int m = (int)(i / quads), n = (int)(i % quads) * 4;
-    const int* src = part + (int64_t)m * ldp + n;
-    i32x4 acc = *(const i32x4*)src;
-#pragma unroll 4
-    for (int z = 1; z < slices; z++) acc += *(const i32x4*)(src + (int64_t)z * p.m * ldp);
-    const float sa = p.a_scale[m];
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-        if (n + e < p.n) sgv_traits<T>::store((T*)p.c + (int64_t)m * p.ldc + n + e, finish(p, acc[e], sa, p.b_scale[n + e], p.bias ? p.bias[n + e] : 0.f));
-}
-
 // ---------------------------------------------------------------------------------------------------------------------------------------
-enum form { ROWS, TILE64, TILE128, TILE256 };
-struct plan { form f; int slices, slice; };
+// Which form serves a product (microseconds in a replayed graph, operands rotating through 3 sets, bf16 out):
+//                            m x n x k           rows kernel   64^2 tiles   128^2    256^2
+//   few rows                 32 x 512 x 8192         5.9           -          -        -        16 x 8192 x 8192: 13.2 (5.1 TB/s), 1 x 8192 x 8192: 12.7 (5.3 TB/s)
+//   few tiles, a long k     100 x 512 x 2048         4.9          6.2         9.4     24.5
+//                           512 x 512 x 2048         5.3          6.5         9.5     24.3
+//   ... a short k           256 x 512 x 512          4.1          4.0         5.3     12.0
+//   some tiles              777 x 1001 x 1030       14.3          5.8         8.0     20.0
+//                           128 x 4096 x 4096       13.4         10.2        22.4     41.3
+//   about a tile per CU    1500 x 1500 x 1500       37.3         14.1        13.6     27.2
+//                          2048 x 2048 x 2048       65.3         18.9        15.1     26.6
+//   many                  10007 x 512 x 512         38.6         11.7         9.2     13.9
+//                          4096 x 4096 x 4096         -          114          76       61
+//                          8192 x 8192 x 8192         -          861         581      470      (2,340 TOP/s)
+enum form { ROWS11, ROWS21, ROWS22, TILE64, TILE128, TILE256 };
 
-static inline int64_t tiles(int m, int n, int edge) { return ((int64_t)(m + edge - 1) / edge) * ((n + edge - 1) / edge); }
+static inline int64_t tiles(int m, int n, int em, int en) { return ((int64_t)(m + em - 1) / em) * ((n + en - 1) / en); }
 
-static plan choose(int m, int n, int k, int64_t lda, int64_t ldb) {
-    const int whole = (k + 127) / 128 * 128;
-    const bool near = lda < (1 << 23) && ldb < (1 << 23);           // the offsets inside a tile fit 32 bits
-    if (m <= 64 || !near) return plan{ROWS, 1, whole};
-    if (tiles(m, n, 256) >= 200) return plan{TILE256, 1, whole};
-    if (tiles(m, n, 128) >= 200) return plan{TILE128, 1, whole};
-    const int64_t t64 = tiles(m, n, 64);
-    const int slices = (int)std::min<int64_t>(256 / t64, whole / 512);
-    if (slices >= 2) {
-        const int slice = (whole / 128 + slices - 1) / slices * 128;
-        return plan{TILE64, (whole + slice - 1) / slice, slice};
-    }
-    return plan{TILE64, 1, whole};
+static form choose(int m, int n, int k) {
+    // few rows: B is read once by as many workgroups as there are; 32 rows take 32 columns where 16 would mean more than one workgroup per CU
+    if (m <= 16) return ROWS11;
+    if (m <= 32) return tiles(m, n, 32, 16) <= 256 ? ROWS21 : ROWS22;
+    // few tiles: the time is the K loop of one of them, which eight waves split
+    if (tiles(m, n, 32, 32) <= 256 && k >= 1024) return ROWS22;
+    // 256 CUs hold two 128^2 tiles each, or one 256^2 tile at 1.6 times the time of two
+    const int64_t t128 = tiles(m, n, 128, 128), t256 = tiles(m, n, 256, 256);
+    if (t128 < 150) return TILE64;
+    return (t256 + 255) / 256 * 1.6 <= (double)((t128 + 511) / 512) ? TILE256 : TILE128;
 }
 
-static inline int64_t partial_pitch(int n) { return ((int64_t)n + 3) / 4 * 4; }
+template <typename T, int MT, int NT, int S>
+static void launch_rows(const args& p, int waves, hipStream_t stream) {
+    const dim3 grid((unsigned)((p.n + 16 * NT - 1) / (16 * NT)), (unsigned)((p.m + 16 * MT - 1) / (16 * MT))), block(64 * waves);
+    const size_t lds = (size_t)waves * std::max(S * (MT + NT) * 2048, MT * NT * 1024);
+    hipLaunchKernelGGL((int8_rows_kernel<T, MT, NT, S>), grid, block, lds, stream, p);
+}
 
 template <typename T, int BM, int BN, int WGM, int WGN, int S, int LEAD>
-static void launch_tile(args p, int slices, hipStream_t stream) {
+static void launch_tile(args p, hipStream_t stream) {
     p.tiles_m = (p.m + BM - 1) / BM;
     p.tiles_n = (p.n + BN - 1) / BN;
-    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WGM, WGN, S, LEAD>), dim3((unsigned)(p.tiles_m * p.tiles_n), (unsigned)slices), dim3(64 * WGM * WGN), 0, stream, p);
+    hipLaunchKernelGGL((int8_tile_kernel<T, BM, BN, WGM, WGN, S, LEAD>), dim3((unsigned)(p.tiles_m * p.tiles_n)), dim3(64 * WGM * WGN), 0, stream, p);
 }
 
 template <typename T>
-static void launch(args p, const plan& pl, void* workspace, hipStream_t stream) {
-    p.slice = pl.slice;
-    if (pl.f == ROWS) {
-        const int mt = p.m <= 16 ? 1 : p.m <= 32 ? 2 : 4;
-        const int steps = (p.k + 63) / 64;
-        const int waves = std::max(1, std::min(mt == 4 ? 8 : 16, steps));
-        const dim3 grid((unsigned)((p.n + 15) / 16), (unsigned)((p.m + 16 * mt - 1) / (16 * mt))), block(64 * waves);
-        const size_t lds = (size_t)waves * mt * 1024;
-        if (mt == 1) hipLaunchKernelGGL((int8_rows_kernel<T, 1, 8>), grid, block, lds, stream, p);
-        else if (mt == 2) hipLaunchKernelGGL((int8_rows_kernel<T, 2, 4>), grid, block, lds, stream, p);
-        else hipLaunchKernelGGL((int8_rows_kernel<T, 4, 4>), grid, block, lds, stream, p);
-    } else if (pl.slices > 1) {
-        args q = p;
-        q.c = workspace;
-        q.ldc = partial_pitch(p.n);
-        launch_tile<int, 64, 64, 2, 2, 4, 1>(q, pl.slices, stream);
-        const int64_t quads = q.ldc / 4 * p.m;
-        hipLaunchKernelGGL((int8_sum_kernel<T>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, stream, p, (const int*)workspace, q.ldc, pl.slices);
-    } else if (pl.f == TILE256) launch_tile<T, 256, 256, 2, 4, 2, 2>(p, 1, stream);
-    else if (pl.f == TILE128) launch_tile<T, 128, 128, 2, 4, 4, 1>(p, 1, stream);
-    else launch_tile<T, 64, 64, 2, 2, 4, 1>(p, 1, stream);
+static void launch(const args& p, form f, hipStream_t stream) {
+    switch (f) {
+        case ROWS11: launch_rows<T, 1, 1, 2>(p, std::min(4, (p.k + 127) / 128), stream); break;
+        case ROWS21: launch_rows<T, 2, 1, 2>(p, std::min(8, (p.k + 127) / 128), stream); break;
+        case ROWS22: launch_rows<T, 2, 2, 2>(p, std::min(8, (p.k + 127) / 128), stream); break;
+        case TILE64: launch_tile<T, 64, 64, 2, 2, 4, 1>(p, stream); break;
+        case TILE128: launch_tile<T, 128, 128, 2, 4, 2, 1>(p, stream); break;
+        case TILE256: launch_tile<T, 256, 256, 2, 4, 2, 2>(p, stream); break;
+    }
 }
 
 }  // namespace sgv_i8
-
-extern "C" int64_t sgv_int8_gemm_workspace_bytes(int32_t m, int32_t n, int32_t k, int64_t lda, int64_t ldb) {
-    if (m < 1 || n < 1 || k < 1 || k > 131071) return 0;
-    const sgv_i8::plan pl = sgv_i8::choose(m, n, k, lda, ldb);
-    return pl.slices > 1 ? (int64_t)pl.slices * m * sgv_i8::partial_pitch(n) * 4 : 0;
-}
 
 extern "C" int sgv_int8_gemm(const sgv_int8_gemm_params* q, int dtype, void* stream_) {
     if (!q) return sgv_fail(SGV_ERR_INVALID_ARG, "int8_gemm: params is NULL");
@@ -391,11 +382,9 @@ extern "C" int sgv_int8_gemm(const sgv_int8_gemm_params* q, int dtype, void* str
     if (((uintptr_t)q->a) % 16 || ((uintptr_t)q->b) % 16 || q->lda % 16 || q->ldb % 16 || q->lda < 0 || q->ldb < 0)
         return sgv_fail(SGV_ERR_INVALID_ARG, "int8_gemm: rows of a and b start on 16 bytes and can be read up to the next multiple of 16 columns");
     if (q->ldc < q->n) return sgv_fail(SGV_ERR_INVALID_ARG, "int8_gemm: rows of c overlap");
-    const sgv_i8::plan pl = sgv_i8::choose(q->m, q->n, q->k, q->lda, q->ldb);
-    if (pl.f == sgv_i8::ROWS && ((int64_t)q->m + 63) / 64 > 65535) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: too many rows");
-    if (sgv_i8::tiles(q->m, q->n, pl.f == sgv_i8::TILE256 ? 256 : pl.f == sgv_i8::TILE128 ? 128 : 64) > 0x7fffffff) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: too many tiles");
-    if (q->workspace_bytes < sgv_int8_gemm_workspace_bytes(q->m, q->n, q->k, q->lda, q->ldb) || (pl.slices > 1 && !q->workspace))
-        return sgv_fail(SGV_ERR_INVALID_ARG, "int8_gemm: this size needs sgv_int8_gemm_workspace_bytes() of workspace");
+    if (q->lda >= 1 << 23 || q->ldb >= 1 << 23) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: rows are at most 8 MB apart (offsets inside a tile are 32 bits)");
+    const sgv_i8::form f = sgv_i8::choose(q->m, q->n, q->k);
+    if (f <= sgv_i8::ROWS22 ? ((int64_t)q->m + 15) / 16 > 65535 : sgv_i8::tiles(q->m, q->n, 64, 64) > 0x7fffffff) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: too many tiles");
     sgv_i8::args p{};
     p.a = (const int8_t*)q->a; p.b = (const int8_t*)q->b; p.a_scale = q->a_scale; p.b_scale = q->b_scale; p.bias = q->bias; p.c = q->c;
     p.lda = q->lda; p.ldb = q->ldb; p.ldc = q->ldc; p.m = q->m; p.n = q->n; p.k = q->k;
@@ -403,8 +392,8 @@ extern "C" int sgv_int8_gemm(const sgv_int8_gemm_params* q, int dtype, void* str
     hipStream_t stream = (hipStream_t)stream_;
     const double m = q->m, n = q->n, k = q->k;
     sgv_launch_scope scope(SGV_K_INT8_GEMM, stream, m * k + n * k + m * n * (double)sgv_dtype_size(dtype), 2.0 * m * n * k);
-    if (dtype == SGV_F32) sgv_i8::launch<float>(p, pl, q->workspace, stream);
-    else if (dtype == SGV_F16) sgv_i8::launch<sgv_half_t>(p, pl, q->workspace, stream);
-    else sgv_i8::launch<sgv_bf16_t>(p, pl, q->workspace, stream);
+    if (dtype == SGV_F32) sgv_i8::launch<float>(p, f, stream);
+    else if (dtype == SGV_F16) sgv_i8::launch<sgv_half_t>(p, f, stream);
+    else sgv_i8::launch<sgv_bf16_t>(p, f, stream);
     return sgv_check_launch("int8_gemm kernel");
 }

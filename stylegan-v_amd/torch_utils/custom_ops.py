@@ -277,7 +277,7 @@ class RmsNormBackwardParams(ctypes.Structure):
 
 class Int8GemmParams(ctypes.Structure):
     _fields_ = [('a', c_void_p), ('b', c_void_p), ('a_scale', c_void_p), ('b_scale', c_void_p), ('bias', c_void_p), ('c', c_void_p),
-                ('workspace', c_void_p), ('workspace_bytes', c_int64), ('lda', c_int64), ('ldb', c_int64), ('ldc', c_int64), ('m', c_int32), ('n', c_int32), ('k', c_int32),
+                ('lda', c_int64), ('ldb', c_int64), ('ldc', c_int64), ('m', c_int32), ('n', c_int32), ('k', c_int32),
                 ('act', c_int32), ('alpha', c_float), ('gain', c_float)]
 
 
@@ -341,7 +341,6 @@ ABI_SYMBOLS = {
     'sgv_rms_norm_backward_workspace_bytes': (c_int64, [c_int64, c_int32, c_int]),
     'sgv_rms_norm_backward': (c_int, [ctypes.POINTER(RmsNormBackwardParams), c_int, c_void_p]),
     'sgv_dequantize_rows': (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int, c_void_p]),
-    'sgv_int8_gemm_workspace_bytes': (c_int64, [c_int32, c_int32, c_int32, c_int64, c_int64]),
     'sgv_int8_gemm': (c_int, [ctypes.POINTER(Int8GemmParams), c_int, c_void_p]),
     'sgv_multi_nan_to_num_f32': (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), c_int32, c_float, c_float, c_float, c_void_p]),
     'sgv_multi_scale_f32': (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), ctypes.POINTER(c_float), c_int32, c_void_p]),

@@ -15,6 +15,7 @@ from . import bias_act as _ba
 from . import rms_norm as _rn
 
 max_inner = 131071     # 128 * 128 * K has to fit in a signed 32-bit sum
+max_stride = 1 << 23   # bytes between two rows that the product takes as they are
 
 
 def quantize_rows(x):
@@ -62,7 +63,7 @@ def _product_rows(q):
     rows, cols = q.shape
     pitch = (cols + 15) // 16 * 16
     stride = q.stride(0) if rows > 1 else pitch
-    if q.data_ptr() % 16 == 0 and stride % 16 == 0 and (cols == pitch or q.storage_offset() + (rows - 1) * stride + pitch <= q.untyped_storage().nbytes()):
+    if q.data_ptr() % 16 == 0 and stride % 16 == 0 and stride < max_stride and (cols == pitch or q.storage_offset() + (rows - 1) * stride + pitch <= q.untyped_storage().nbytes()):
         return q, stride
     out = torch.empty([rows, pitch], dtype=torch.int8, device=q.device)
     out[:, :cols].copy_(q)          # (what lies behind the last column is ignored)
@@ -108,10 +109,8 @@ def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype
         bc = bias.contiguous() if bias is not None else None
         lib = custom_ops.get_native()
         m = ar.shape[0]
-        size = lib.sgv_int8_gemm_workspace_bytes(m, n, cols, lda, ldb)
-        work = torch.empty([size], dtype=torch.uint8, device=a.device) if size else None
         p = custom_ops.Int8GemmParams(ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), bc.data_ptr() if bc is not None else None, out.data_ptr(),
-                                      work.data_ptr() if size else None, size, lda, ldb, n, m, n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
+                                      lda, ldb, n, m, n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
         with custom_ops.device_guard(a):
             custom_ops.check(lib.sgv_int8_gemm(p, _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(a)), lib)
     return out

@@ -101,8 +101,10 @@ def test_argument_checks_of_the_c_entry_without_gpu():
     assert lib.sgv_int8_gemm(p, F32, None) == -1
     p.lda, p.ldc = 32, 0
     assert lib.sgv_int8_gemm(p, F32, None) == -1 and b'overlap' in lib.sgv_last_error()
-    p.ldc = 1
+    p.ldc, p.lda = 1, 1 << 23
+    assert lib.sgv_int8_gemm(p, F32, None) == -2 and b'apart' in lib.sgv_last_error()
+    p.lda = 32
     assert lib.sgv_int8_gemm(p, custom_ops.SGV_F64, None) == -3
     p.m = 0
     assert lib.sgv_int8_gemm(p, F32, None) == 0
-    assert ctypes.sizeof(custom_ops.Int8GemmParams) == 112
+    assert ctypes.sizeof(custom_ops.Int8GemmParams) == 96

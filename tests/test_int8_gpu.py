@@ -42,7 +42,7 @@ def _verify(got, a, sa, b, sb, bias, act, gain, dtype):
 
 SIZES = [(1, 1, 1), (1, 512, 512), (1, 1000, 8192), (2, 17, 16), (7, 33, 15), (15, 16, 64), (16, 16, 65), (17, 64, 63), (32, 512, 8192), (33, 31, 129), (64, 100, 1000), (65, 130, 17),
          (100, 513, 48), (127, 128, 128), (128, 127, 2047), (129, 257, 2048), (200, 300, 2049), (255, 256, 100), (256, 255, 4096), (257, 300, 333), (511, 1025, 1030), (513, 512, 512),
-         (1000, 1001, 1003), (1025, 520, 144), (2049, 1000, 272), (3000, 2100, 640)]
+         (1000, 1001, 1003), (1025, 520, 144), (2049, 1000, 272), (3000, 2100, 640), (2600, 2600, 300), (4100, 4200, 200)]
 
 
 @pytest.mark.parametrize('m,n,k', SIZES)
@@ -76,7 +76,7 @@ def test_extreme_bytes_and_longest_sums(m, n):
 
 def test_strides_alignments_and_shapes():
     base, wb = _bytes(70, 400, 1), _bytes(90, 400, 2)
-    for cut in (lambda t: t[:, 16:336], lambda t: t[:, 1:300], lambda t: t[:, :39], lambda t: t[::2, 32:], lambda t: t[:, ::2], lambda t: t[5:6], lambda t: t[1:2].expand(40, 400),
+    for cut in (lambda t: t[:, 16:336],  lambda t: t[:, 1:300], lambda t: t[:, :39], lambda t: t[::2, 32:], lambda t: t[:, ::2], lambda t: t[5:6], lambda t: t[1:2].expand(40, 400),
                 lambda t: t[:64].t(), lambda t: t[-3:, -33:], lambda t: t.as_strided([20, 48], [16, 1])):
         a, b = cut(base), cut(wb)
         sa, sb = _scales(a.shape[0], 1), _scales(b.shape[0], 2)
@@ -88,6 +88,16 @@ def test_strides_alignments_and_shapes():
     assert int8.matmul(base[:0], sa.view(70)[:0], wb, sb).shape == (0, 90) and int8.matmul(base, sa.view(70), wb[:0], sb[:0]).shape == (70, 0)
     sliced = int8.matmul(base, _scales(140, 1)[::2], wb, _scales(180, 2)[::2])          # scales with strides
     assert torch.equal(sliced, int8.matmul(base, _scales(140, 1)[::2].contiguous(), wb, _scales(180, 2)[::2].contiguous()))
+
+
+def test_rows_far_apart_and_overlapping():
+    base = torch.zeros([40 << 20], dtype=torch.int8, device=DEV)
+    base.random_(-128, 128, generator=torch.Generator(device=DEV).manual_seed(0))
+    for rows, stride in ((4, (1 << 23) - 16), (4, 1 << 23), (4, (1 << 23) + 16), (2, 36 << 20), (300, 131072), (300, 16), (300, 0)):
+        a, b = base.as_strided([rows, 200], [stride, 1]), _bytes(70, 200, 1)
+        sa, sb = _scales(rows, 2), _scales(70, 3)
+        _verify(int8.matmul(a, sa, b, sb), a, sa, b, sb, None, 'linear', 1.0, torch.float32)
+        _verify(int8.matmul(b, sb, a, sa), b, sb, a, sa, None, 'linear', 1.0, torch.float32)
 
 
 def test_a_row_does_not_depend_on_its_batch():
