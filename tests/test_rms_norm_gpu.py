@@ -110,7 +110,7 @@ def test_many_rows_weight_gradient(rows, cols):
     dx, dw = torch.autograd.grad(rn.rms_norm(x, w), (x, w), dy)
     _, hd, inv, _ = _exact(x.detach(), None, None, 1e-8)
     t = dy.double() * hd * inv
-    # a thread adds at most rows / 512 + 4 rows (one workgroup takes every 512th), then 4 waves, then 512 / 16 partial sums and 16 waves
+    # a thread adds at most rows / 512 + 4 rows (one workgroup takes every 512th), then 4 waves, then 1024 / 64 partial sums and 6 levels
     _check(dw, t.sum(dim=0), t.abs().sum(dim=0), 44 + rows / 512 + 4 + 4 + 32 + 16, 'dw')
     again = torch.autograd.grad(rn.rms_norm(x, w), (x, w), dy)
     assert torch.equal(again[0], dx) and torch.equal(again[1], dw)          # a fixed order: the same bits
