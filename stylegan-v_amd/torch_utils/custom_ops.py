@@ -19,6 +19,7 @@ import ctypes
 import hashlib
 import os
 import shutil
+import struct
 import subprocess
 import threading
 from concurrent.futures import ThreadPoolExecutor
@@ -386,11 +387,11 @@ class device_guard:
     __slots__ = ('idx', 'prev')
 
     def __init__(self, tensor):
-        self.idx = tensor.device.index
+        self.idx = tensor.get_device()
 
     def __enter__(self):
         import torch
-        self.prev = torch.cuda.current_device()
+        self.prev = torch._C._cuda_getDevice()      # (torch.cuda.current_device() without its look at the lazy initialisation: the tensor is on a device)
         if self.prev != self.idx:
             torch.cuda.set_device(self.idx)
 
@@ -399,6 +400,37 @@ class device_guard:
             import torch
             torch.cuda.set_device(self.prev)
         return False
+
+
+class PackedEntry:
+    """An entry point `int f(const block*, int dtype, void* stream)` called with the fields of its parameter block as plain values (pointers as integers, 0 for none), on
+    the current stream of a tensor's device.  For operators whose kernels take as long as their launch shim: packing the fields into bytes and passing those takes
+    0.8 us of host time, filling a ctypes.Structure and passing it 2.3 us."""
+    _CODES = {c_void_p: 'Q', c_int64: 'q', c_int32: 'i', c_float: 'f'}
+
+    def __init__(self, name, block):
+        self.name, self.block, self.fn = name, block, None
+
+    def _bind(self):
+        import torch
+        pack = struct.Struct('@' + ''.join(self._CODES[t] for _, t in self.block._fields_))
+        fields = [getattr(self.block, name) for name, _ in self.block._fields_]
+        assert pack.size <= ctypes.sizeof(self.block) < pack.size + 8 and fields[-1].offset + fields[-1].size == pack.size     # (native alignment: the compiler's, less the padding behind the last field)
+        fn = get_native()[self.name]         # a function object of its own: the shared one takes the structure
+        fn.restype, fn.argtypes = c_int, [ctypes.c_char_p, c_int, c_void_p]
+        self.pack, self.device, self.stream, self.fn = pack.pack, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, fn
+
+    def __call__(self, tensor, dtype, *fields):
+        if self.fn is None:
+            self._bind()
+        idx = tensor.get_device()
+        if self.device() == idx:
+            rc = self.fn(self.pack(*fields), dtype, self.stream(idx))
+        else:
+            with device_guard(tensor):
+                rc = self.fn(self.pack(*fields), dtype, self.stream(idx))
+        if rc:
+            check(rc)
 
 
 def launch_count():

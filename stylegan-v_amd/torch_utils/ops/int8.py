@@ -14,6 +14,7 @@ from .. import custom_ops
 from . import bias_act as _ba
 from . import rms_norm as _rn
 
+_gemm = custom_ops.PackedEntry('sgv_int8_gemm', custom_ops.Int8GemmParams)
 max_inner = 131071     # 128 * 128 * K has to fit in a signed 32-bit sum
 max_stride = 1 << 23   # bytes between two rows that the product takes as they are
 
@@ -39,13 +40,14 @@ def dequantize_rows(q, scale, dtype=torch.float32):
     _rn.check_no_grad('dequantize_rows', scale)
     if not q.is_cuda:
         return (q.float() * scale.unsqueeze(-1)).to(dtype)
+    out = q.new_empty(q.shape, dtype=dtype)
     rows = _rn.row_view(q)
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
     if rows.shape[0]:
+        scale = _rn._dense(scale)
         lib = custom_ops.get_native()
         with custom_ops.device_guard(q):
-            custom_ops.check(lib.sgv_dequantize_rows(rows.data_ptr(), rows.stride(0) if rows.shape[0] > 1 else 0, scale.contiguous().data_ptr(), out.data_ptr(), rows.shape[0], rows.shape[1],
-                                                     _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(q)), lib)
+            custom_ops.check(lib.sgv_dequantize_rows(rows.data_ptr(), rows.stride(0), scale.data_ptr(), out.data_ptr(), rows.shape[0], rows.shape[1], _rn._DTYPE_CODES[dtype],
+                                                     custom_ops.raw_stream(q)), lib)
     return out
 
 
@@ -57,17 +59,17 @@ def _check_rows(what, name, q, scale):
 
 
 def _product_rows(q):
-    """(tensor to keep, row stride in bytes): the rows of q starting on 16 bytes and readable up to the next multiple of 16 columns -- q itself where it is so (what
+    """(tensor to keep, rows, row stride in bytes): the rows of q starting on 16 bytes and readable up to the next multiple of 16 columns -- q itself where it is so (what
     ``quantize_rows`` and ``rms_norm_int8`` return, and any dense K % 16 == 0 tensor), else a copy."""
     q = _rn.row_view(q)
     rows, cols = q.shape
     pitch = (cols + 15) // 16 * 16
     stride = q.stride(0) if rows > 1 else pitch
-    if q.data_ptr() % 16 == 0 and stride % 16 == 0 and stride < max_stride and (cols == pitch or q.storage_offset() + (rows - 1) * stride + pitch <= q.untyped_storage().nbytes()):
-        return q, stride
-    out = torch.empty([rows, pitch], dtype=torch.int8, device=q.device)
+    if stride % 16 == 0 and stride < max_stride and q.data_ptr() % 16 == 0 and (cols == pitch or q.storage_offset() + (rows - 1) * stride + pitch <= q.untyped_storage().nbytes()):
+        return q, rows, stride
+    out = q.new_empty((rows, pitch))
     out[:, :cols].copy_(q)          # (what lies behind the last column is ignored)
-    return out, pitch
+    return out, rows, pitch
 
 
 def _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype):
@@ -97,22 +99,17 @@ def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype
         raise RuntimeError('matmul: bias must be fp32, one element per row of b, on the device of a')
     _rn.check_no_grad('matmul', a_scale, b_scale, bias)
     spec = _ba.activation_funcs[act]
-    gain = float(spec.def_gain if act_gain is None else act_gain)
+    gain = spec.def_gain if act_gain is None else act_gain
     if not a.is_cuda:
         return _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype)
     n = b.shape[0]
-    out = torch.empty(a.shape[:-1] + (n,), dtype=dtype, device=a.device)
+    out = a.new_empty(a.shape[:-1] + (n,), dtype=dtype)
     if out.numel():
-        ar, lda = _product_rows(a)
-        br, ldb = _product_rows(b)
-        sa, sb = a_scale.contiguous(), b_scale.contiguous()
-        bc = bias.contiguous() if bias is not None else None
-        lib = custom_ops.get_native()
-        m = ar.shape[0]
-        p = custom_ops.Int8GemmParams(ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), bc.data_ptr() if bc is not None else None, out.data_ptr(),
-                                      lda, ldb, n, m, n, cols, spec.cuda_idx, float(spec.def_alpha), gain)
-        with custom_ops.device_guard(a):
-            custom_ops.check(lib.sgv_int8_gemm(p, _rn._DTYPE_CODES[dtype], custom_ops.raw_stream(a)), lib)
+        ar, m, lda = _product_rows(a)
+        br, _, ldb = _product_rows(b)
+        sa, sb, bc = _rn._dense(a_scale), _rn._dense(b_scale), _rn._dense(bias)
+        _gemm(a, _rn._DTYPE_CODES[dtype], ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), _rn._ptr(bc), out.data_ptr(), lda, ldb, n, m, n, cols, spec.cuda_idx,
+              spec.def_alpha, gain)
     return out
 
 

@@ -18,6 +18,8 @@ import torch
 
 from .. import custom_ops
 
+_forward = custom_ops.PackedEntry('sgv_rms_norm', custom_ops.RmsNormParams)
+_backward = custom_ops.PackedEntry('sgv_rms_norm_backward', custom_ops.RmsNormBackwardParams)
 _DTYPE_CODES = {torch.float32: custom_ops.SGV_F32, torch.float16: custom_ops.SGV_F16, torch.bfloat16: custom_ops.SGV_BF16}
 
 
@@ -29,21 +31,24 @@ def check_no_grad(what, *tensors):
 def _check(what, x, weight, residual, eps):
     if not isinstance(x, torch.Tensor) or x.ndim < 1 or x.shape[-1] < 1:
         raise RuntimeError(f'{what}: x must be a tensor of rows (at least one dimension, the last one not empty)')
-    if x.dtype not in _DTYPE_CODES and not (x.dtype == torch.float64 and not x.is_cuda):
-        raise RuntimeError(f'{what}: unsupported dtype {x.dtype}')
+    dtype = x.dtype
+    if dtype not in _DTYPE_CODES and not (dtype == torch.float64 and not x.is_cuda):
+        raise RuntimeError(f'{what}: unsupported dtype {dtype}')
     if not eps >= 0:
         raise RuntimeError(f'{what}: eps must be >= 0')
     if weight is not None:
         if weight.ndim != 1 or weight.shape[0] != x.shape[-1]:
             raise RuntimeError(f'{what}: weight must have one element per column')
-        if weight.dtype not in (x.dtype, torch.float32) or weight.device != x.device:
+        if (weight.dtype != dtype and weight.dtype != torch.float32) or weight.device != x.device:
             raise RuntimeError(f'{what}: weight must have the type of x or fp32, on the device of x')
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+    if residual is not None and (residual.shape != x.shape or residual.dtype != dtype or residual.device != x.device):
         raise RuntimeError(f'{what}: residual must have the same shape, dtype, and device as x')
 
 
 def row_view(t):
     """t as [rows, columns] with unit stride along a row: a view where t allows one, else a copy."""
+    if t.is_contiguous():
+        return t if t.ndim == 2 else t.view(-1, t.shape[-1])
     cols = t.shape[-1]
     if t.ndim != 2:
         t = t.reshape(-1, cols)
@@ -53,49 +58,46 @@ def row_view(t):
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return 0 if t is None else t.data_ptr()
 
 
 def _stride(t):
-    return t.stride(0) if t is not None and t.shape[0] > 1 else 0
+    return 0 if t is None else t.stride(0)
+
+
+def _dense(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def launch_forward(x, weight, residual, eps, int8, normalize=True, want_inv=False):
-    """(y or q, h or None, inv_rms or None, scale or None), all as rows; x and residual: ``row_view``s on a GPU."""
+    """(y or q, h or None, inv_rms or None, scale or None), all as rows; x and residual: ``row_view``s on a GPU, weight dense."""
     rows, cols = x.shape
-    dev = x.device
-    h = torch.empty([rows, cols], dtype=x.dtype, device=dev) if residual is not None else None
-    inv = torch.empty([rows], dtype=torch.float32, device=dev) if want_inv else None
+    h = None if residual is None else x.new_empty((rows, cols))
+    inv = x.new_empty(rows, dtype=torch.float32) if want_inv else None
     if int8:      # rows on 16 bytes, zeros behind the last column: what the 8-bit product reads
         pitch = (cols + 15) // 16 * 16
-        y, scale = torch.empty([rows, pitch], dtype=torch.int8, device=dev), torch.empty([rows], dtype=torch.float32, device=dev)
+        y, scale = x.new_empty((rows, pitch), dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
     else:
         pitch = cols
-        y, scale = torch.empty([rows, cols], dtype=x.dtype, device=dev), None
+        y, scale = x.new_empty((rows, cols)), None
     if rows:
-        lib = custom_ops.get_native()
-        p = custom_ops.RmsNormParams(x.data_ptr(), _ptr(residual), _ptr(weight), None if int8 else y.data_ptr(), _ptr(h), _ptr(inv), y.data_ptr() if int8 else None, _ptr(scale),
-                                     rows, _stride(x), _stride(residual), pitch, cols, int(weight is not None and weight.dtype == torch.float32), int(normalize), eps)
-        with custom_ops.device_guard(x):
-            custom_ops.check(lib.sgv_rms_norm(p, _DTYPE_CODES[x.dtype], custom_ops.raw_stream(x)), lib)
+        out = y.data_ptr()
+        _forward(x, _DTYPE_CODES[x.dtype], x.data_ptr(), _ptr(residual), _ptr(weight), 0 if int8 else out, _ptr(h), _ptr(inv), out if int8 else 0, _ptr(scale), rows, _stride(x),
+                 _stride(residual), pitch, cols, weight is not None and weight.dtype == torch.float32, normalize, eps)
     return (y[:, :cols] if pitch != cols else y), h, inv, scale
 
 
 def _launch_backward(dy, h, dh, weight, inv, need_dx, need_dw):
     rows, cols = h.shape
-    dev = h.device
-    dx = torch.empty([rows, cols], dtype=h.dtype, device=dev) if need_dx else None
-    dw = torch.empty([cols], dtype=weight.dtype, device=dev) if need_dw else None
+    dx = h.new_empty((rows, cols)) if need_dx else None
+    dw = torch.empty_like(weight) if need_dw else None
     if rows == 0:
         return dx, (dw.zero_() if need_dw else None)
-    lib = custom_ops.get_native()
     code = _DTYPE_CODES[h.dtype]
-    size = lib.sgv_rms_norm_backward_workspace_bytes(rows, cols, code) if need_dw else 0
-    work = torch.empty([size // 4], dtype=torch.float32, device=dev) if need_dw else None
-    p = custom_ops.RmsNormBackwardParams(dy.data_ptr(), h.data_ptr(), _ptr(dh), _ptr(weight), inv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(work), size, rows, _stride(dy), _stride(h),
-                                         _stride(dh), cols, int(weight is not None and weight.dtype == torch.float32))
-    with custom_ops.device_guard(h):
-        custom_ops.check(lib.sgv_rms_norm_backward(p, code, custom_ops.raw_stream(h)), lib)
+    size = custom_ops.get_native().sgv_rms_norm_backward_workspace_bytes(rows, cols, code) if need_dw else 0
+    work = inv.new_empty(size // 4) if need_dw else None
+    _backward(h, code, dy.data_ptr(), h.data_ptr(), _ptr(dh), _ptr(weight), inv.data_ptr(), _ptr(dx), _ptr(dw), _ptr(work), size, rows, _stride(dy), _stride(h), _stride(dh), cols,
+              weight is not None and weight.dtype == torch.float32)
     return dx, dw
 
 
@@ -134,16 +136,15 @@ class _RmsNormFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, residual, eps):
-        w = weight.contiguous() if weight is not None else None
-        y, h, inv, _ = launch_forward(x, w, residual, eps, int8=False, want_inv=True)
-        ctx.eps, ctx.has_residual = eps, residual is not None
+        y, h, inv, _ = launch_forward(x, _dense(weight), residual, eps, int8=False, want_inv=True)
+        ctx.eps, ctx.inv = eps, inv
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x if residual is None else h, weight, inv)
+        ctx.save_for_backward(x if residual is None else h, weight)
         return y if residual is None else (y, h)
 
     @staticmethod
     def backward(ctx, dy, dh=None):
-        h, weight, inv = ctx.saved_tensors
+        h, weight = ctx.saved_tensors
         need_dx = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
         need_dw = ctx.needs_input_grad[1] and dy is not None
         if torch.is_grad_enabled():
@@ -152,7 +153,7 @@ class _RmsNormFn(torch.autograd.Function):
             dx, dw = dh, None
         else:
             rows = [t if t is None or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous() for t in (dy, dh)]
-            dx, dw = _launch_backward(rows[0], h, rows[1], weight.contiguous() if weight is not None else None, inv, need_dx, need_dw)
+            dx, dw = _launch_backward(rows[0], h, rows[1], _dense(weight), ctx.inv, need_dx, need_dw)
         return (dx if ctx.needs_input_grad[0] else None), (dw if need_dw else None), (dx if ctx.needs_input_grad[2] else None), None
 
 
@@ -161,7 +162,12 @@ def rms_norm(x, weight=None, residual=None, eps=1e-8):
     _check('rms_norm', x, weight, residual, eps)
     if not x.is_cuda:
         return rms_norm_ref(x, weight, residual, eps)
-    out = _RmsNormFn.apply(row_view(x), weight, row_view(residual) if residual is not None else None, float(eps))
+    rows, res = row_view(x), None if residual is None else row_view(residual)
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)):
+        out = _RmsNormFn.apply(rows, weight, res, eps)
+    else:
+        out = launch_forward(rows, _dense(weight), res, eps, int8=False)
+        out = out[0] if residual is None else out[:2]
     if x.ndim == 2:
         return out
     return out.view(x.shape) if residual is None else (out[0].view(x.shape), out[1].view(x.shape))
@@ -188,7 +194,7 @@ def rms_norm_int8(x, weight=None, residual=None, eps=1e-8):
         factor = (u.square().mean(dim=-1, keepdim=True) + eps).rsqrt()
         q, scale = quantize_ref(u if weight is None else u * weight.double(), factor)
         return (q, scale) if residual is None else (q, scale, h)
-    q, h, _, scale = launch_forward(row_view(x), weight.contiguous() if weight is not None else None, row_view(residual) if residual is not None else None, float(eps), int8=True)
+    q, h, _, scale = launch_forward(row_view(x), _dense(weight), None if residual is None else row_view(residual), eps, int8=True)
     if x.ndim != 2:
         q, scale = q.unflatten(0, x.shape[:-1]) if x.ndim > 2 else q[0], scale.view(x.shape[:-1])
         h = h.view(x.shape) if h is not None else None
