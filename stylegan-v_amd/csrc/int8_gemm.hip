@@ -384,7 +384,10 @@ extern "C" int sgv_int8_gemm(const sgv_int8_gemm_params* q, int dtype, void* str
     if (q->ldc < q->n) return sgv_fail(SGV_ERR_INVALID_ARG, "int8_gemm: rows of c overlap");
     if (q->lda >= 1 << 23 || q->ldb >= 1 << 23) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: rows are at most 8 MB apart (offsets inside a tile are 32 bits)");
     const sgv_i8::form f = sgv_i8::choose(q->m, q->n, q->k);
-    if (f <= sgv_i8::ROWS22 ? ((int64_t)q->m + 15) / 16 > 65535 : sgv_i8::tiles(q->m, q->n, 64, 64) > 0x7fffffff) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: too many tiles");
+    // (a launch has fewer than 2^32 threads)
+    const int64_t threads = f == sgv_i8::ROWS11 ? sgv_i8::tiles(q->m, q->n, 16, 16) * 256 : f <= sgv_i8::ROWS22 ? sgv_i8::tiles(q->m, q->n, 32, 16) * 512
+                          : f == sgv_i8::TILE64 ? sgv_i8::tiles(q->m, q->n, 64, 64) * 256 : sgv_i8::tiles(q->m, q->n, f == sgv_i8::TILE128 ? 128 : 256, f == sgv_i8::TILE128 ? 128 : 256) * 512;
+    if (threads >= 1ll << 32) return sgv_fail(SGV_ERR_TOO_LARGE, "int8_gemm: too many tiles");
     sgv_i8::args p{};
     p.a = (const int8_t*)q->a; p.b = (const int8_t*)q->b; p.a_scale = q->a_scale; p.b_scale = q->b_scale; p.bias = q->bias; p.c = q->c;
     p.lda = q->lda; p.ldb = q->ldb; p.ldc = q->ldc; p.m = q->m; p.n = q->n; p.k = q->k;

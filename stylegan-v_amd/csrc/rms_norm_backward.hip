@@ -114,10 +114,10 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_ker
     }
 }
 
-// rows beyond the registers: two walks; a workgroup's weight-gradient sums live in its own row of `partials`
-template <typename T>
-__global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(const bwd_args p) {
-    constexpr int VEC = io<T>::VEC, TEAM = 1024;
+// rows that are not held in registers: two walks; a workgroup's weight-gradient sums live in its own row of `partials`
+template <typename T, int TEAM>
+__global__ __launch_bounds__(TEAM) void rms_norm_backward_long_kernel(const bwd_args p) {
+    constexpr int VEC = io<T>::VEC;
     __shared__ red_slots red;
     int turn = 0;
     float* out = p.partials ? p.partials + (int64_t)blockIdx.x * p.cols : nullptr;
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(const bwd_
         const T* dh = p.dh ? (const T*)p.dh + row * p.dh_stride : nullptr;
         const float inv = p.inv_rms[row];
         const bool first = row == (int64_t)blockIdx.x;
-        float c = 0.f;
+        double along = 0.0;
         for (int i = threadIdx.x * VEC; i < p.cols; i += TEAM * VEC) {
             float g[VEC], xh[VEC], w[VEC];
             io<T>::unpack(load_vec<T, true>(dy, i, p.cols), g);
@@ -137,10 +137,10 @@ __global__ __launch_bounds__(1024) void rms_norm_backward_long_kernel(const bwd_
             for (int j = 0; j < VEC; j++) {
                 xh[j] *= inv;
                 if (out && i + j < p.cols) out[i + j] = first ? g[j] * xh[j] : __builtin_fmaf(g[j], xh[j], out[i + j]);
-                c = __builtin_fmaf(g[j] * w[j], xh[j], c);
+                along += (double)(g[j] * w[j]) * xh[j];
             }
         }
-        c = team_sum<TEAM>(c, red, turn) * p.inv_cols;
+        const float c = (float)(team_wide<TEAM>(along, red, turn, add_op()) / p.cols);
         if (p.dx)
             for (int i = threadIdx.x * VEC; i < p.cols; i += TEAM * VEC) {
                 float g[VEC], xh[VEC], w[VEC], e[VEC];
@@ -185,7 +185,8 @@ static void launch_backward(const bwd_args& p, const shape& s, int64_t blocks, h
 }
 template <typename T>
 static void launch_backward(const bwd_args& p, const shape& s, int64_t blocks, hipStream_t stream) {
-    if (s.team == 0) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
+    if (s.elems == 0 && s.team == 64) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T, 64>), dim3((unsigned)blocks), dim3(64), 0, stream, p);
+    else if (s.elems == 0) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T, 1024>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
     else if (p.partials) { if (p.stream) launch_backward<T, true, true>(p, s, blocks, stream); else launch_backward<T, false, true>(p, s, blocks, stream); }
     else { if (p.stream) launch_backward<T, true, false>(p, s, blocks, stream); else launch_backward<T, false, false>(p, s, blocks, stream); }
 }
@@ -201,7 +202,7 @@ extern "C" int sgv_rms_norm_backward(const sgv_rms_norm_backward_params* q, int 
     if (!q) return sgv_fail(SGV_ERR_INVALID_ARG, "rms_norm_backward: params is NULL");
     if (!sgv_rn::row_dtype(dtype)) return sgv_fail(SGV_ERR_UNSUPPORTED, "rms_norm_backward: rows are fp32, fp16 or bf16");
     if (q->rows < 1 || q->cols < 1) return sgv_fail(SGV_ERR_INVALID_ARG, "rms_norm_backward: rows and cols must be >= 1");
-    if (q->cols > 0x7fffffff - 16384) return sgv_fail(SGV_ERR_TOO_LARGE, "rms_norm_backward: rows are too long");
+    if (q->cols > sgv_rn::MAX_COLS) return sgv_fail(SGV_ERR_TOO_LARGE, "rms_norm_backward: rows are too long");
     if (!q->dy || !q->h || !q->inv_rms || (!q->dx && !q->dweight)) return sgv_fail(SGV_ERR_INVALID_ARG, "rms_norm_backward: NULL pointer");
     if (q->dweight && !q->weight) return sgv_fail(SGV_ERR_INVALID_ARG, "rms_norm_backward: a gradient of no weight");
     if (q->dy_stride < 0 || q->h_stride < 0 || q->dh_stride < 0) return sgv_fail(SGV_ERR_INVALID_ARG, "rms_norm_backward: negative strides");

@@ -234,20 +234,23 @@ struct held_weight {
     }
 };
 
-// How a row is held: TEAM threads with at most 16 elements each, or not at all (team = 0: rows beyond 16384 elements, and rows shorter than a vector)
+// How a row is held: TEAM threads with at most 16 elements each, or not at all (elems = 0, the walking kernels: one wave for rows shorter than a vector, 1024 threads for
+// rows beyond 16384 elements)
 struct shape { int team, elems; };
 static inline shape row_shape(int cols, int vec) {
     static const shape held[] = {{64, 4}, {64, 8}, {64, 16}, {128, 16}, {256, 16}, {512, 16}, {1024, 16}};
-    if (cols >= vec)
-        for (const shape& s : held) if (s.elems >= vec && cols <= s.team * s.elems) return s;
-    return shape{0, 0};
+    if (cols < vec) return shape{64, 0};
+    for (const shape& s : held) if (s.elems >= vec && cols <= s.team * s.elems) return s;
+    return shape{1024, 0};
 }
+constexpr int MAX_COLS = (1 << 26) - 1;          // (the launch that adds up the weight gradient has 64 threads for a column)
 
 // Workgroups of a launch: twice as many as the CUs hold at once (2048 threads each), which walk over the rows.  With a weight gradient they are the rows of its partial
 // sums, which should stay small beside the rows: as many as the CUs hold at once, four rows to each at least ([2049, 1111] fp16: 13.4 us with two).
 static inline int64_t groups(int64_t rows, const shape& s, bool dw) {
-    const int64_t teams = s.team == 64 ? (rows + 3) / 4 : rows;
-    const int threads = s.team == 0 ? 1024 : s.team == 64 ? 256 : s.team;
+    const bool four = s.team == 64 && s.elems > 0;       // four rows to a workgroup
+    const int64_t teams = four ? (rows + 3) / 4 : rows;
+    const int threads = four ? 256 : s.team;
     const int64_t most = dw ? std::min<int64_t>(std::max(512, 131072 / threads), std::max<int64_t>(256, rows / 4)) : 512 * (2048 / threads);
     return std::min(teams, most);
 }

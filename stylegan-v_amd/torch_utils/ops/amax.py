@@ -32,6 +32,11 @@ def graph_replayed():
     _epoch += 1
 
 
+def replay_epoch():
+    """How many times `graph_replayed` was called: part of the state that anything derived from parameters was derived at, beside their version counters."""
+    return _epoch
+
+
 _ARENA = 4096
 _arenas = {}       # device index -> [zeroed fp32 tensor, slots handed out]
 SINK_SLOTS = 4096              # SGV_AMAX_SINK_SLOTS of include/sgv_ops.h

@@ -81,40 +81,57 @@ def _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype):
     return (v * gain).to(dtype)
 
 
+def _check_layer(what, cols, device, b, b_scale, bias, dtype, act):
+    _check_rows(what, 'b', b, b_scale)
+    if b.ndim != 2 or b.shape[1] != cols or b.device != device:
+        raise RuntimeError(f'{what}: b must be [N, K] with the K of a, on the device of a')
+    if cols > max_inner:
+        raise RuntimeError(f'{what}: K is at most {max_inner} (a sum of 128 * 128 * K has to fit in 32 bits)')
+    if dtype not in _rn._DTYPE_CODES:
+        raise RuntimeError(f'{what}: unsupported dtype {dtype}')
+    if act not in ('linear', 'lrelu'):
+        raise RuntimeError(f'{what}: unsupported activation {act}')
+    if bias is not None and (bias.ndim != 1 or bias.shape[0] != b.shape[0] or bias.dtype != torch.float32 or bias.device != device):
+        raise RuntimeError(f'{what}: bias must be fp32, one element per row of b, on the device of a')
+
+
+def _launch(a, m, lda, a_scale, b, b_scale, bias, act, act_gain, out):
+    """out = the product of the rows of a (dense scales) with the rows of b."""
+    n, cols = b.shape
+    br, _, ldb = _product_rows(b)
+    sb, bc = _rn._dense(b_scale), _rn._dense(bias)
+    spec = _ba.activation_funcs[act]
+    _gemm(out, _rn._DTYPE_CODES[out.dtype], a.data_ptr(), br.data_ptr(), a_scale.data_ptr(), sb.data_ptr(), _rn._ptr(bc), out.data_ptr(), lda, ldb, n, m, n, cols, spec.cuda_idx,
+          spec.def_alpha, spec.def_gain if act_gain is None else act_gain)
+    return out
+
+
 def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype=torch.float32):
     """a [..., K] int8 with a_scale [...], b [N, K] int8 with b_scale [N], bias [N] or None -> [..., N] in ``dtype`` (fp32, fp16, bf16).
     ``act``: 'linear' or 'lrelu'; ``act_gain``: its gain (default: the activation's own, sqrt(2) for lrelu)."""
     _check_rows('matmul', 'a', a, a_scale)
-    _check_rows('matmul', 'b', b, b_scale)
-    cols = a.shape[-1]
-    if b.ndim != 2 or b.shape[1] != cols or b.device != a.device:
-        raise RuntimeError('matmul: b must be [N, K] with the K of a, on the device of a')
-    if cols > max_inner:
-        raise RuntimeError(f'matmul: K is at most {max_inner} (a sum of 128 * 128 * K has to fit in 32 bits)')
-    if dtype not in _rn._DTYPE_CODES:
-        raise RuntimeError(f'matmul: unsupported dtype {dtype}')
-    if act not in ('linear', 'lrelu'):
-        raise RuntimeError(f'matmul: unsupported activation {act}')
-    if bias is not None and (bias.ndim != 1 or bias.shape[0] != b.shape[0] or bias.dtype != torch.float32 or bias.device != a.device):
-        raise RuntimeError('matmul: bias must be fp32, one element per row of b, on the device of a')
+    _check_layer('matmul', a.shape[-1], a.device, b, b_scale, bias, dtype, act)
     _rn.check_no_grad('matmul', a_scale, b_scale, bias)
-    spec = _ba.activation_funcs[act]
-    gain = spec.def_gain if act_gain is None else act_gain
     if not a.is_cuda:
-        return _matmul_ref(a, a_scale, b, b_scale, bias, act, gain, dtype)
-    n = b.shape[0]
-    out = a.new_empty(a.shape[:-1] + (n,), dtype=dtype)
+        return _matmul_ref(a, a_scale, b, b_scale, bias, act, _ba.activation_funcs[act].def_gain if act_gain is None else act_gain, dtype)
+    out = a.new_empty(a.shape[:-1] + b.shape[:1], dtype=dtype)
     if out.numel():
-        ar, m, lda = _product_rows(a)
-        br, _, ldb = _product_rows(b)
-        sa, sb, bc = _rn._dense(a_scale), _rn._dense(b_scale), _rn._dense(bias)
-        _gemm(a, _rn._DTYPE_CODES[dtype], ar.data_ptr(), br.data_ptr(), sa.data_ptr(), sb.data_ptr(), _rn._ptr(bc), out.data_ptr(), lda, ldb, n, m, n, cols, spec.cuda_idx,
-              spec.def_alpha, gain)
+        rows, m, lda = _product_rows(a)
+        _launch(rows, m, lda, _rn._dense(a_scale), b, b_scale, bias, act, act_gain, out)
     return out
 
 
 def dense(x, weight, weight_scale, bias=None, act='linear', act_gain=None, normalize=False, eps=1e-8):
     """x [..., K] fp32 / fp16 / bf16, weight [N, K] int8 with weight_scale [N] (``quantize_rows`` of the layer's weight), bias [N] fp32 -> [..., N] in x's type.
     ``normalize``: the rows of x through ``rms_norm`` (no weight) first, in the same pass that quantises them."""
-    q, scale = _rn.rms_norm_int8(x, eps=eps) if normalize else quantize_rows(x)
-    return matmul(q, scale, weight, weight_scale, bias=bias, act=act, act_gain=act_gain, dtype=x.dtype)
+    if not x.is_cuda:
+        q, scale = _rn.rms_norm_int8(x, eps=eps) if normalize else quantize_rows(x)
+        return matmul(q, scale, weight, weight_scale, bias=bias, act=act, act_gain=act_gain, dtype=x.dtype)
+    _rn._check('dense', x, None, None, eps)
+    _check_layer('dense', x.shape[-1], x.device, weight, weight_scale, bias, x.dtype, act)
+    _rn.check_no_grad('dense', x, weight_scale, bias)
+    out = x.new_empty(x.shape[:-1] + weight.shape[:1])
+    if out.numel():
+        q, _, _, scale = _rn.launch_forward(_rn.row_view(x), None, None, eps, int8=True, normalize=normalize)
+        _launch(q, q.shape[0], q.stride(0), scale, weight, weight_scale, bias, act, act_gain, out)
+    return out

@@ -16,7 +16,7 @@ import torch
 import torch.nn.functional as F
 
 from ..torch_utils import misc
-from ..torch_utils.ops import bias_act, conv2d_gradfix, conv2d_resample, eqlr, fc, fused_conv_act, fused_down_act, int8, pointwise, upfirdn2d
+from ..torch_utils.ops import amax, bias_act, conv2d_gradfix, conv2d_resample, eqlr, fc, fused_conv_act, fused_down_act, int8, pointwise, upfirdn2d
 
 
 @misc.profiled_function
@@ -34,37 +34,36 @@ class FullyConnectedLayer(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.full([out_features], float(bias_init))) if bias else None
         self.weight_gain = lr_multiplier / math.sqrt(in_features)
         self.bias_gain = lr_multiplier
-        for name in ('weight_int8', 'weight_int8_scale', 'bias_int8'):      # (not in the state dict: derived from the parameters by quantize_int8_)
-            self.register_buffer(name, None, persistent=False)
-        self._int8_of = None
+        self._int8 = None       # (weight rows, their scales, bias, state of the parameters) of quantize_int8_: derived from the parameters, neither buffers nor state
 
-    def _parameter_versions(self):
-        return tuple(None if p is None or p.is_inference() else p._version for p in (self.weight, self.bias))
+    def _parameter_state(self):
+        return tuple((p.device, p.dtype, None if p.is_inference() else p._version) for p in (self.weight, self.bias) if p is not None) + (amax.replay_epoch(),)
 
     def quantize_int8_(self):
         """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
-        quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters change
-        afterwards (an optimiser step, ``load_state_dict``) refuses to serve until it is quantised again.  Returns the layer."""
+        quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters changed or moved
+        since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``) refuses to serve until it is quantised again.  Returns the layer."""
         if self.activation not in ('linear', 'lrelu'):
             raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
         with torch.no_grad():
-            self.weight_int8, self.weight_int8_scale = int8.quantize_rows(self.weight.float() * self.weight_gain)
-            self.bias_int8 = self.bias.float() * self.bias_gain if self.bias is not None else None
-        self._int8_of = self._parameter_versions()
+            rows, scales = int8.quantize_rows(self.weight.detach().float() * self.weight_gain)
+            bias = self.bias.detach().float() * self.bias_gain if self.bias is not None else None
+        self._int8 = (rows, scales, bias, self._parameter_state())
         return self
 
     def serves_int8(self):
-        return self.weight_int8 is not None and not torch.is_grad_enabled()
+        return self._int8 is not None and not torch.is_grad_enabled()
 
     def forward(self, x, normalize_input=False, gain=None):
         """``normalize_input``: apply normalize_2nd_moment to x first (the mapping network's first layer; one kernel with the layer).
         ``gain``: the layer's output times a constant (ToRGB's ``affine(w) * weight_gain``, networks.py:314) -- rides on the kernel's activation gain instead of
         costing a launch here and another in the backward pass."""
         if self.serves_int8():
-            if self._parameter_versions() != self._int8_of:
+            rows, scales, bias, state = self._int8
+            if state != self._parameter_state():
                 raise RuntimeError('the parameters of this layer changed after quantize_int8_(): quantise it again')
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
-            return int8.dense(x, self.weight_int8, self.weight_int8_scale, self.bias_int8, act=self.activation, act_gain=act_gain, normalize=normalize_input)
+            return int8.dense(x, rows, scales, bias, act=self.activation, act_gain=act_gain, normalize=normalize_input)
         if x.ndim == 2:   # one kernel on the GPU (ops/fc.py -> csrc/fc.hip); the torch composition elsewhere
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
             return fc.dense(x, self.weight, self.bias, weight_gain=self.weight_gain, bias_gain=self.bias_gain, act=self.activation, normalize=normalize_input, act_gain=act_gain)

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from stylegan_v_amd.torch_utils import custom_ops
-from stylegan_v_amd.torch_utils.ops import int8
+from stylegan_v_amd.torch_utils.ops import amax, int8
 from stylegan_v_amd.training.layers import FullyConnectedLayer, MappingNetwork
 
 
@@ -66,6 +66,13 @@ def test_layer_serves_in_8_bits_without_gradients_only():
         with pytest.raises(RuntimeError, match='quantise it again'):
             layer(x)
         layer.quantize_int8_()(x)
+        layer.quantize_int8_()
+        amax.graph_replayed()                             # a replayed graph may have written the parameters behind their version counters
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            layer(x)
+        assert layer.quantize_int8_().bfloat16()._int8 is not None
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            layer(x)
     with pytest.raises(RuntimeError, match='tanh'):
         FullyConnectedLayer(4, 4, activation='tanh').quantize_int8_()
 
@@ -80,6 +87,23 @@ def test_mapping_network_in_8_bits():
     assert got.shape == want.shape
     # three layers, each with two operands off by up to half a step of 1/127 of a row's maximum: ~ 3 * sqrt(2) * (max / rms ~ 3) * 1/127/sqrt(12) = 3 % of the result's size
     assert (got - want).norm() / want.norm() < 0.06
+
+
+def test_training_goes_on_beside_a_served_average():
+    """The averaged generator served in 8 bits inside a training process: the steps run, and the average refuses to serve numbers of an older state."""
+    from stylegan_v_amd.training import config as cfgs, train_step
+    g_kwargs, d_kwargs = cfgs.small_test_model_kwargs(res=32)
+    cfg = cfgs.Config(r1_gamma=1.0, lr=0.0025, betas=(0.0, 0.99), ema_kimg=1.0, ema_rampup=0.05, G_reg_interval=4, D_reg_interval=16, pl_weight=0.0)
+    ts = train_step.TrainStep(g_kwargs, d_kwargs, cfg, device='cpu', batch_gpu=2)
+    z, c, keys = torch.randn([2, 32]), torch.zeros([2, 0]), set(ts.G_ema.state_dict())
+    with torch.no_grad():
+        ts.G_ema.mapping.quantize_int8_()(z, c)
+    ts.step()
+    assert set(ts.G_ema.state_dict()) == keys
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            ts.G_ema.mapping(z, c)
+        ts.G_ema.mapping.quantize_int8_()(z, c)
 
 
 def test_argument_checks_of_the_c_entry_without_gpu():

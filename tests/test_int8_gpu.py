@@ -157,7 +157,8 @@ def test_mapping_network_served_in_8_bits(batch):
         x = z.cpu()
         for i in range(2):
             fc = getattr(net, f'fc{i}')
-            x = int8.dense(x, fc.weight_int8.cpu(), fc.weight_int8_scale.cpu(), fc.bias_int8.cpu(), act='lrelu', normalize=(i == 0))
+            rows, scales, bias, _ = fc._int8
+            x = int8.dense(x, rows.cpu(), scales.cpu(), bias.cpu(), act='lrelu', normalize=(i == 0))
     # the fp32 sums between the layers differ by a few U, which moves a value across a border of its 8-bit grid now and then: one step, 1/127 of a row's largest value,
     # in one of its 512 columns; the whole result stays within a hundredth of that
     assert (got[:, 0].cpu() - x).norm() / x.norm() < 1e-3

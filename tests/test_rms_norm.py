@@ -99,7 +99,7 @@ def test_argument_checks_of_the_c_entries_without_gpu():
     assert lib.sgv_rms_norm(p, F32, None) == -1 and b'eps' in lib.sgv_last_error()
     p.eps = 0.0
     assert lib.sgv_rms_norm(p, custom_ops.SGV_F64, None) == -3
-    p.cols = 0x7fffffff
+    p.cols = 1 << 26
     assert lib.sgv_rms_norm(p, F32, None) == -2
     p.rows, p.cols = 0, 8
     assert lib.sgv_rms_norm(p, F32, None) == 0                          # nothing to do

@@ -103,7 +103,7 @@ def test_forward_gradient_and_8_bits(cols, dtype):
 
 
 @pytest.mark.parametrize('rows', [1, 2, 5, 511, 2047, 2049, 5000])
-@pytest.mark.parametrize('cols', [24, 520, 2900])
+@pytest.mark.parametrize('cols', [3, 24, 520, 2900])
 def test_many_rows_weight_gradient(rows, cols):
     x, w, dy = _rand(rows, cols, seed=rows), _rand(cols, seed=1), _rand(rows, cols, seed=rows + 2)
     x, w = x.requires_grad_(True), w.requires_grad_(True)
