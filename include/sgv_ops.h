@@ -543,7 +543,7 @@ int sgv_multi_scale_f32(const float* const* src, float* const* dst, const int64_
  * normalize = 0 (8-bit output only): y = h * weight -- the plain quantisation of rows.
  * Rows are fp32, fp16 or bf16 (`dtype`) with unit stride along a row; x_stride / residual_stride: elements between rows (0: one row for all); y and h are dense.
  * Rows of q start on 16 bytes; columns from `cols` up to the next multiple of 16 are written with zeros.
- * inv_rms [rows] (optional): rsqrt(mean h^2 + eps), what the backward pass takes. */
+ * inv_rms [rows] (optional): rsqrt(mean h^2 + eps), what the backward pass takes.  Outputs must not overlap inputs.  cols < 2^26. */
 typedef struct sgv_rms_norm_params {
     const void* x; const void* residual; const void* weight;
     void* y; void* h; float* inv_rms;

@@ -3,9 +3,12 @@
 //   C[m,n] = act( (sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n] ) * gain        A [M,K], B [N,K] signed bytes, sums in 32-bit integers
 //
 // Both operands are contiguous along k, which is how the matrix instruction wants them: a lane of v_mfma_i32_16x16x64_i8 holds 16 consecutive bytes of one row
-// (row = lane & 15, bytes 16 (lane >> 4) ..+15 of 64).  The integer sums are exact whatever their order, so K is split freely -- over the waves of a workgroup, over
-// workgroups -- and the result depends neither on the split nor on the other rows of a batch.
+// (row = lane & 15, bytes 16 (lane >> 4) ..+15 of 64).  The integer sums are exact whatever their order, so K is split freely over the waves of a workgroup, and the result
+// depends neither on the split nor on the other rows of a batch.
 //
+// Two kernels: int8_rows_kernel for few rows (bound by reading B once: 1 x 8192 x 8192 12.7 us = 5.3 TB/s) and few tiles, int8_tile_kernel for the rest (bound by the matrix
+// pipe's power: 8192^3 464 us = 2,370 TOP/s at 1.5 GHz, where the chip holds 2.4 GHz without load; 0.63 of the issue slots).  The table at choose() below has
+// both sides of every border.
 #include "sgv_common.h"
 
 #include <algorithm>
@@ -47,7 +50,8 @@ __device__ __forceinline__ float finish(const args& p, int acc, float sa, float 
 // Tiles of C.  K is walked in stages of 128 bytes per row -- a cache line -- that go from memory straight into LDS (buffer_load ... lds: no registers, no instructions
 // to store them), S stages in a ring.  A stage's 16-byte chunks lie at position chunk ^ ((row >> 1) & 7) of their row, which makes the fragment reads below free of
 // bank conflicts.  A wave holds the fragments of one step of 64 k in registers and replaces each as soon as its last product is issued, so that the matrix pipe finds
-// the next step's fragments there; one barrier per stage.  Rows beyond the matrix and bytes beyond its end are outside the buffers' bounds and read as zero.
+// the next step's fragments there; one barrier per stage.  (16x16x64 rather than 32x32x32 products: half the accumulator traffic for the same work, 557 -> 527 us at
+// 8192^3, where time is energy.  128 bytes of K per stage rather than 64: whole cache lines, 500 -> 477 us.)  Rows beyond the matrix and bytes beyond its end are outside the buffers' bounds and read as zero.
 
 __device__ __forceinline__ i32x4 make_rsrc(const void* base, int64_t bytes) {
     const uint64_t b = (uint64_t)base;
@@ -62,7 +66,7 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff, i
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // Few tiles: every wave of a workgroup computes the whole 16 MT x 16 NT tile over its own stages of K (128 bytes per row; wave w takes stages w, w + waves, ...), in a
 // ring of S stages of LDS of its own -- no barrier in the loop --, and the waves' sums meet in LDS.  Through LDS because the matrix instruction wants 16 rows side by side:
-// read straight into registers, 16 neighbouring lanes touch 16 cache lines, and a CU gets 16 bytes a clock instead of 64 (32 x 512 x 8192: 13.0 us).
+// read straight into registers, 16 neighbouring lanes touch 16 cache lines, and a CU gets 16 bytes a clock instead of 64 (32 x 512 x 8192: 13.0 us against 5.9).
 template <typename T, int MT, int NT, int S>
 __global__ __launch_bounds__(512) void int8_rows_kernel(const args p) {
     extern __shared__ __attribute__((aligned(128))) int8_t ring[];          // [waves][S][(MT + NT) * 16 rows][128], then [waves][MT * NT * 256] sums
@@ -239,8 +243,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
         for (int i = 0; i < LEAD; i++) row(i);
         __builtin_amdgcn_sched_barrier(0);
         if (cross) {
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "n"((S - 2) * LPS) : "memory");
-            __builtin_amdgcn_s_barrier();
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"((S - 2) * LPS) : "memory");
         }
 #pragma unroll
         for (int i = 0; i < LEAD; i++) fa[i] = *(const i32x4*)(s + abase + i * 16 * BK + c);
@@ -260,8 +263,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
 #pragma unroll
         for (int j = 0; j < TN; j++) fb[j] = fn[j];
     };
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"((S - 1) * LPS) : "memory");
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" :: "n"((S - 1) * LPS) : "memory");
 #pragma unroll
     for (int j = 0; j < TN; j++) fb[j] = *(const i32x4*)(lds + bbase + j * 16 * BK + ck[0]);
 #pragma unroll
@@ -287,8 +289,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
     static_assert(WAVES * 16 * PITCH <= S * STAGE && (16 * CH) % 64 == 0, "");
 #pragma unroll
     for (int i = 0; i < PER; i++) { const int x = i * 64 * WAVES + threadIdx.x; if (x < BN) { sb_lds[x] = sbv[i]; bias_lds[x] = biv[i]; } }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");            // (every load into LDS has landed, the empty ones too: the ring may be written over)
-    __builtin_amdgcn_s_barrier();
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // (every load into LDS has landed, the empty ones too: the ring may be written over)
     int8_t* buf = lds + wave * 16 * PITCH;
     const int nb = n0 + wn * TN * 16;
     const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;

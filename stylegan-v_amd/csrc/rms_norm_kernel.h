@@ -6,12 +6,16 @@
 //   8 bits: u = h * w,  q = rint_half_even(127 u / max|u|),  scale = max|y| / 127   (inv cancels out of q)
 //   gradient, with g = dy * w and xh = h * inv:  dx = dr = inv * (g - xh * mean_k(g xh)) + dh,   dw = sum_rows dy * xh
 //
-// All of it is bound by memory (12 operations per element against 3..10 bytes): a row is read once into registers, 16 bytes per lane and load, and nothing is
-// read again.  Rows of up to 4 vectors per lane of a wave are one wave's (no barrier at all), longer ones a 256-thread workgroup's, and rows beyond the registers of
-// one take a kernel that walks the row three times (its second and third reads come from the L2).  16-byte accesses need no alignment on this chip, so odd
-// lengths and strides take the same kernels; only a row's last, partial vector is read element by element.
+// All of it is bound by memory (12 operations per element against 3..10 bytes): a row is read once into registers, 16 bytes per lane and load, at most 16 elements to a
+// thread, and nothing is read again.  Rows of up to 1024 elements are one wave's (no barrier at all), longer ones a workgroup's of 128..1024 threads; workgroups walk
+// over rows with the next row's loads in flight while one is reduced and written, and hold the weight in registers.  Rows beyond 16384 elements are walked over
+// three times (the later reads come from the L2).  16-byte accesses need no alignment on this chip, so odd lengths and strides take the same kernels: a row's last,
+// partial vector is moved back to end with the row.  Calls that move more than the caches hold go past them.
+// Measured (a 1 GB copy: 5.2 TB/s): [16384, 4096] bf16 forward 42 us = 6.3 TB/s, with a residual 93 us = 5.8, to 8 bits with a residual 76 us = 6.2, backward with all
+// gradients 93 us = 5.8; [30000, 1111] fp16 forward 23 us = 5.7, backward 71 us = 3.7 (rows off the cache lines).  Rows to 8 bits without a residual are the exception:
+// 16-bit rows run at 3.8..4.3 TB/s, bound by the instructions of the rounding.
 //
-// Statistics are fp32: a lane sums at most 64 squares before the tree.  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a tiny eps) is
+// Statistics are fp32: a lane sums at most 16 squares before the tree (fp64 in the walking kernels).  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a tiny eps) is
 // summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 4e-5 of a step, so a value within 5e-5 of a border
 // between two steps is decided by the fp64 quotient; the row maximum is exact because the product of two 16-bit values is exact in fp32, and other products are
 // taken in fp64.

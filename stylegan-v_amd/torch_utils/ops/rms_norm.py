@@ -24,8 +24,10 @@ _DTYPE_CODES = {torch.float32: custom_ops.SGV_F32, torch.float16: custom_ops.SGV
 
 
 def check_no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f'{what} serves inference and has no gradient: call it under torch.no_grad() or with detached tensors')
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f'{what} serves inference and has no gradient: call it under torch.no_grad() or with detached tensors')
 
 
 def _check(what, x, weight, residual, eps):
@@ -145,16 +147,19 @@ class _RmsNormFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy, dh=None):
         h, weight = ctx.saved_tensors
-        need_dx = ctx.needs_input_grad[0] or ctx.needs_input_grad[2]
-        need_dw = ctx.needs_input_grad[1] and dy is not None
+        need_x, need_w, need_r, _ = ctx.needs_input_grad
+        need_w = need_w and dy is not None
         if torch.is_grad_enabled():
             dx, dw = _gradient_ref(dy, h, dh, weight, ctx.eps)
         elif dy is None:
             dx, dw = dh, None
         else:
-            rows = [t if t is None or t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous() for t in (dy, dh)]
-            dx, dw = _launch_backward(rows[0], h, rows[1], _dense(weight), ctx.inv, need_dx, need_dw)
-        return (dx if ctx.needs_input_grad[0] else None), (dw if need_dw else None), (dx if ctx.needs_input_grad[2] else None), None
+            if dy.stride(1) != 1 and dy.shape[1] != 1:
+                dy = dy.contiguous()
+            if dh is not None and dh.stride(1) != 1 and dh.shape[1] != 1:
+                dh = dh.contiguous()
+            dx, dw = _launch_backward(dy, h, dh, _dense(weight), ctx.inv, need_x or need_r, need_w)
+        return (dx if need_x else None), (dw if need_w else None), (dx if need_r else None), None
 
 
 def rms_norm(x, weight=None, residual=None, eps=1e-8):
