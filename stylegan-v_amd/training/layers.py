@@ -27,6 +27,10 @@ def normalize_2nd_moment(x, dim=1, eps=1e-8):
 class FullyConnectedLayer(torch.nn.Module):
     """Equalised-learning-rate dense layer: weight stored as randn/lr_mul, used as W*lr_mul/sqrt(in)."""
 
+    # (weight rows, their scales, bias, state of the parameters, their storage) of quantize_int8_: derived from the parameters, neither buffers nor state.  On the class, so
+    # that layers unpickled from before the attribute existed have it too
+    _int8 = None
+
     def __init__(self, in_features, out_features, bias=True, activation='linear', lr_multiplier=1, bias_init=0):
         super().__init__()
         self.activation = activation
@@ -34,21 +38,23 @@ class FullyConnectedLayer(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.full([out_features], float(bias_init))) if bias else None
         self.weight_gain = lr_multiplier / math.sqrt(in_features)
         self.bias_gain = lr_multiplier
-        self._int8 = None       # (weight rows, their scales, bias, state of the parameters) of quantize_int8_: derived from the parameters, neither buffers nor state
 
     def _parameter_state(self):
-        return tuple((p.device, p.dtype, None if p.is_inference() else p._version) for p in (self.weight, self.bias) if p is not None) + (amax.replay_epoch(),)
+        return tuple((p.device, p.dtype, p.data_ptr(), None if p.is_inference() else p._version) for p in (self.weight, self.bias) if p is not None) + (amax.replay_epoch(),)
 
     def quantize_int8_(self):
         """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
         quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters changed or moved
-        since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``) refuses to serve until it is quantised again.  Returns the layer."""
+        since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``, a new ``.data``) refuses to serve until it is quantised again, and so does a copy
+        of the layer.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place writes under inference mode) are not seen, and a captured
+        graph keeps the weight it was captured with.  Returns the layer."""
         if self.activation not in ('linear', 'lrelu'):
             raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
         with torch.no_grad():
             rows, scales = int8.quantize_rows(self.weight.detach().float() * self.weight_gain)
             bias = self.bias.detach().float() * self.bias_gain if self.bias is not None else None
-        self._int8 = (rows, scales, bias, self._parameter_state())
+        held = [p.detach() for p in (self.weight, self.bias) if p is not None]       # (as long as they live, no other tensor gets the addresses in the state)
+        self._int8 = (rows, scales, bias, self._parameter_state(), held)
         return self
 
     def serves_int8(self):
@@ -59,10 +65,12 @@ class FullyConnectedLayer(torch.nn.Module):
         ``gain``: the layer's output times a constant (ToRGB's ``affine(w) * weight_gain``, networks.py:314) -- rides on the kernel's activation gain instead of
         costing a launch here and another in the backward pass."""
         if self.serves_int8():
-            rows, scales, bias, state = self._int8
+            rows, scales, bias, state, _ = self._int8
             if state != self._parameter_state():
                 raise RuntimeError('the parameters of this layer changed after quantize_int8_(): quantise it again')
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
+            if normalize_input and x.ndim != 2:
+                x, normalize_input = normalize_2nd_moment(x), False      # (over dimension 1, whatever the shape)
             return int8.dense(x, rows, scales, bias, act=self.activation, act_gain=act_gain, normalize=normalize_input)
         if x.ndim == 2:   # one kernel on the GPU (ops/fc.py -> csrc/fc.hip); the torch composition elsewhere
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)

@@ -7,7 +7,7 @@ import torch
 
 from stylegan_v_amd.torch_utils import custom_ops
 from stylegan_v_amd.torch_utils.ops import amax, int8
-from stylegan_v_amd.training.layers import FullyConnectedLayer, MappingNetwork
+from stylegan_v_amd.training.layers import FullyConnectedLayer, MappingNetwork, normalize_2nd_moment
 
 
 def _rows(m, k, seed):
@@ -60,8 +60,12 @@ def test_layer_serves_in_8_bits_without_gradients_only():
     with torch.no_grad():
         assert torch.allclose(layer(x, gain=3.0), got * 3.0, rtol=1e-6)
         assert layer(x.view(2, 3, 24)).shape == (2, 3, 10)
-        twin = copy.deepcopy(layer)
-        assert torch.equal(twin(x), got)
+        twin = copy.deepcopy(layer)                       # a copy has parameters of its own
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            twin(x)
+        assert torch.equal(twin.quantize_int8_()(x), got)
+        volume = torch.randn([2, 24, 24])                 # the input norm runs over dimension 1, with three dimensions too
+        assert torch.equal(layer(volume, normalize_input=True), layer(normalize_2nd_moment(volume)))
         layer.weight.add_(0.1)
         with pytest.raises(RuntimeError, match='quantise it again'):
             layer(x)
@@ -70,6 +74,16 @@ def test_layer_serves_in_8_bits_without_gradients_only():
         amax.graph_replayed()                             # a replayed graph may have written the parameters behind their version counters
         with pytest.raises(RuntimeError, match='quantise it again'):
             layer(x)
+        layer.quantize_int8_()
+        layer.weight.data = layer.weight.data * 2         # (a new tensor behind the parameter leaves its version as it was)
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            layer(x)
+        layer.quantize_int8_().half().float()             # (... and so does a round trip through another type)
+        with pytest.raises(RuntimeError, match='quantise it again'):
+            layer(x)
+        old = copy.deepcopy(layer)
+        old.__dict__.pop('_int8', None)                   # a layer from before it had an 8-bit form
+        assert old(x).shape == (6, 10)
         assert layer.quantize_int8_().bfloat16()._int8 is not None
         with pytest.raises(RuntimeError, match='quantise it again'):
             layer(x)

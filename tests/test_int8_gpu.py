@@ -157,7 +157,7 @@ def test_mapping_network_served_in_8_bits(batch):
         x = z.cpu()
         for i in range(2):
             fc = getattr(net, f'fc{i}')
-            rows, scales, bias, _ = fc._int8
+            rows, scales, bias = fc._int8[:3]
             x = int8.dense(x, rows.cpu(), scales.cpu(), bias.cpu(), act='lrelu', normalize=(i == 0))
     # the fp32 sums between the layers differ by a few U, which moves a value across a border of its 8-bit grid now and then: one step, 1/127 of a row's largest value,
     # in one of its 512 columns; the whole result stays within a hundredth of that
