@@ -47,6 +47,9 @@
  *                          weight gradients; the unfolded trajectory convolutions of motion.py:18-156 at thousands of rows
  *   sgv_fc             <- `FullyConnectedLayer.forward` src/training/layers.py:108-138 (weight gain, bias gain, addmm / matmul, bias_act),
  *                          `normalize_2nd_moment` layers.py:16-18, and through unfolded rows `EqLRConv1d` of motion.py
+ *   sgv_rms_norm, sgv_rms_norm_backward (+ _workspace_bytes), sgv_dequantize_rows
+ *                      <- `normalize_2nd_moment` layers.py:16-18 as an operator of its own, with a weight, a residual stream and an 8-bit output
+ *   sgv_int8_gemm      <- `FullyConnectedLayer.forward` layers.py:108-138 with operands quantised to 8 bits (no counterpart in the reference: serving)
  *   sgv_multi_nan_to_num_f32
  *                      <- the `misc.nan_to_num(param.grad, nan=0, posinf=1e5, neginf=-1e5, out=param.grad)` loop of
  *                          src/training/training_loop.py:384-386 as one launch over the whole gradient list
@@ -577,7 +580,8 @@ int sgv_dequantize_rows(const void* q, int64_t q_stride, const float* scale, voi
  * Matrix product in 8-bit integers (csrc/int8_gemm.hip): the dense layer of layers.py:108-138 on quantised rows.
  *   C[m,n] = act( (sum_k A[m,k] B[n,k]) * a_scale[m] * b_scale[n] + bias[n] ) * gain       C in `dtype` (fp32, fp16, bf16), sums in 32-bit integers (exact)
  * Rows of a [m,k] and b [n,k] are signed bytes, start on 16 bytes (base and lda / ldb; rows may overlap, 0: one row for all) and can be READ up to the next multiple of 16 columns: what lies there
- * is ignored (sgv_rms_norm writes its 8-bit rows that way).  k <= 131071.  bias (fp32) may be NULL.  Rows are at most 8 MB apart. */
+ * is ignored (sgv_rms_norm writes its 8-bit rows that way).  k <= 131071.  bias (fp32) may be NULL.  Rows are at most 8 MB apart.  The sum times b_scale has to stay
+ * within fp32's range (b_scale up to 1e29); a_scale may be anything. */
 typedef struct sgv_int8_gemm_params {
     const void* a; const void* b; const float* a_scale; const float* b_scale; const float* bias; void* c;
     int64_t lda, ldb, ldc;

@@ -40,8 +40,9 @@ __device__ __forceinline__ i32x4 mask_tail(i32x4 v, int left) {
     return v;
 }
 
+// (the scale of B first: a weight's is moderate, and rows of any size then leave fp32's range only where the result does)
 __device__ __forceinline__ float finish(const args& p, int acc, float sa, float sb, float bias) {
-    float v = __builtin_fmaf((float)acc * sa, sb, bias);
+    float v = __builtin_fmaf((float)acc * sb, sa, bias);
     if (p.lrelu) v = v > 0.f ? v : v * p.alpha;
     return v * p.gain;
 }

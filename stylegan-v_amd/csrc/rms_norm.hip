@@ -187,7 +187,8 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
     }
 }
 
-// Rows that are not held in registers -- longer than a workgroup's, or shorter than a vector (a wave's): TEAM threads walk over the row once per step.  With a residual, the later walks read the h that the same thread wrote.
+// Rows that are not held in registers -- longer than a workgroup's, or shorter than a vector (a wave's): TEAM threads walk over the row once per step.  With a residual,
+// the later walks read the h that the same thread wrote.
 template <typename T, bool OUT8, int TEAM>
 __global__ __launch_bounds__(TEAM) void rms_norm_long_kernel(const args p) {
     constexpr int VEC = io<T>::VEC;

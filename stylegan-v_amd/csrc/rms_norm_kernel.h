@@ -15,8 +15,8 @@
 // gradients 93 us = 5.8; [30000, 1111] fp16 forward 23 us = 5.7, backward 71 us = 3.7 (rows off the cache lines).  Rows to 8 bits without a residual are the exception:
 // 16-bit rows run at 3.8..4.3 TB/s, bound by the instructions of the rounding.
 //
-// Statistics are fp32: a lane sums at most 16 squares before the tree (fp64 in the walking kernels).  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a tiny eps) is
-// summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 4e-5 of a step, so a value within 5e-5 of a border
+// Statistics are fp32: a lane sums at most 16 squares before the tree (fp64 in the walking kernels).  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a
+// tiny eps) is summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 4e-5 of a step, so a value within 5e-5 of a border
 // between two steps is decided by the fp64 quotient; the row maximum is exact because the product of two 16-bit values is exact in fp32, and other products are
 // taken in fp64.
 #pragma once
@@ -81,10 +81,10 @@ template <> struct io<sgv_bf16_t> {
     }
 };
 
-// The VEC elements of a row at column i; TAIL: a row's length is no multiple of VEC, and elements at or behind `cols` read as zero.
-// The same past the caches (aligned rows only: partial lines are written twice that way)
+// 16 bytes past the caches (aligned rows only: partial lines are written twice that way)
 template <typename T> __device__ __forceinline__ u32x4 stream_vec(const T* row, int i) { return __builtin_nontemporal_load((const u32x4*)(row + i)); }
 template <typename T> __device__ __forceinline__ void stream_vec(T* row, int i, const u32x4& v) { __builtin_nontemporal_store(v, (u32x4*)(row + i)); }
+// The VEC elements of a row at column i; TAIL: a row's length is no multiple of VEC, and elements at or behind `cols` read as zero.
 template <typename T, bool TAIL>
 __device__ __forceinline__ u32x4 load_vec(const T* row, int i, int cols) {
     constexpr int VEC = io<T>::VEC;

@@ -1,6 +1,6 @@
 """8-bit product (csrc/int8_gemm.hip through ops/int8.py) against 64-bit arithmetic, and the operators together as they are served.
 
-The sums are whole numbers and exact.  The epilogue in fp32 (U = 2^-24): one rounding each for the sum as a float, times a_scale, times b_scale plus bias, times the
+The sums are whole numbers and exact.  The epilogue in fp32 (U = 2^-24): one rounding each for the sum as a float, times b_scale, times a_scale plus bias, times the
 slope and the gain (both constants rounded too): 3 U of |sum * scales| and 5 U of the result, then half a step of the output's type."""
 import pytest
 import torch
@@ -116,6 +116,15 @@ def test_scales_that_are_not_numbers():
     keep = torch.ones(40, dtype=torch.bool, device=DEV)
     keep[4] = False
     assert not torch.isfinite(got[keep][:, 7]).any() and torch.isfinite(got[keep][:, :7]).all() and not got[9, :7].any()
+
+
+@pytest.mark.parametrize('m,n,k', [(1, 40, 8192), (3, 512, 512), (40, 70, 2048), (300, 520, 600), (2100, 2000, 512)])
+def test_rows_of_any_size(m, n, k):
+    """Rows up to the end of fp32's range: the result is finite where its value is, whatever the sum times the row's scale would be."""
+    a, b, sa, sb = _bytes(m, k, 1), _bytes(n, k, 2), _scales(m, 3), _scales(n, 4) * 1e-6
+    sa[::3] *= 1e36                                       # a sum is ~ 74^2 sqrt(k) ~ 1e5: 1e39 with this scale, and 1e31 with both
+    sa[1::3] *= 1e-30
+    _verify(int8.matmul(a, sa, b, sb), a, sa, b, sb, None, 'linear', 1.0, torch.float32)
 
 
 def test_refusals_on_the_gpu():
