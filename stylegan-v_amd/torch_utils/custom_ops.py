@@ -17,10 +17,12 @@ which shells out to nvcc through ``torch.utils.cpp_extension.load``.  Difference
 import contextlib
 import ctypes
 import hashlib
+import importlib.machinery
+import importlib.util
 import os
 import shutil
-import struct
 import subprocess
+import sys
 import threading
 from concurrent.futures import ThreadPoolExecutor
 
@@ -177,6 +179,83 @@ def get_native(build=True):
 
 def native_loaded():
     return _lib is not None
+
+
+# The torch side of the operators that take less time on the GPU than Python takes to call them (csrc/row_ops.cpp): host code against torch's headers, beside the
+# library and calling it.
+ROW_OPS_SOURCE = os.path.join(CSRC_DIR, 'row_ops.cpp')
+ROW_OPS_PATH = os.path.join(CSRC_DIR, '_sgv_row_ops.so')
+_ROW_OPS_HASH_PATH = ROW_OPS_PATH + '.md5'
+_ROW_OPS_ENTRIES = ['sgv_rms_norm', 'sgv_rms_norm_backward', 'sgv_rms_norm_backward_workspace_bytes', 'sgv_dequantize_rows', 'sgv_int8_gemm', 'sgv_last_error']
+_row_ops = None
+_row_ops_error = None
+
+
+def row_ops_digest():
+    import torch
+    md5 = hashlib.md5(('%s %s' % (torch.__version__, sys.version)).encode())      # (built against this torch and this interpreter)
+    for path in (ROW_OPS_SOURCE, os.path.join(INCLUDE_DIR, 'sgv_ops.h')):
+        with open(path, 'rb') as fh:
+            md5.update(fh.read())
+    return md5.hexdigest()
+
+
+def row_ops_built():
+    if not (os.path.isfile(ROW_OPS_PATH) and os.path.isfile(_ROW_OPS_HASH_PATH)):
+        return False
+    with open(_ROW_OPS_HASH_PATH) as fh:
+        return fh.read().strip() == row_ops_digest()
+
+
+def build_row_ops(force=False):
+    """Compile csrc/row_ops.cpp in-tree.  Returns the .so path."""
+    import sysconfig
+    import torch
+    with _lock, _build_file_lock():
+        if not force and row_ops_built():
+            return ROW_OPS_PATH
+        root = os.path.dirname(torch.__file__)
+        rocm = os.path.dirname(os.path.dirname(os.path.realpath(_hipcc())))
+        include = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'), os.path.join(rocm, 'include'), sysconfig.get_paths()['include']]
+        tmp = ROW_OPS_PATH + '.tmp.%d' % os.getpid()
+        cmd = ([shutil.which('g++') or 'g++', '-O2', '-std=c++17', '-fPIC', '-fvisibility=hidden', '-shared', '-D__HIP_PLATFORM_AMD__=1', '-DUSE_ROCM=1',
+                '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch._C._GLIBCXX_USE_CXX11_ABI] + ['-I' + p for p in include]
+               + [ROW_OPS_SOURCE, '-o', tmp, '-L' + os.path.join(root, 'lib'), '-lc10', '-ltorch_cpu', '-ltorch', '-ltorch_python', '-lc10_hip'])
+        if verbosity != 'none':
+            print('[sgv] building %s...' % os.path.basename(ROW_OPS_PATH), flush=True)
+        if verbosity == 'full':
+            print(' '.join(cmd))
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise NativeLibraryError('g++ failed for %s:\n%s' % (ROW_OPS_SOURCE, res.stderr[-4000:]))
+        os.replace(tmp, ROW_OPS_PATH)
+        with open(_ROW_OPS_HASH_PATH, 'w') as fh:
+            fh.write(row_ops_digest())
+        return ROW_OPS_PATH
+
+
+def get_row_ops():
+    """The loaded module of csrc/row_ops.cpp, bound to the library; built first if it is stale or missing.  Raises NativeLibraryError (cached) if it cannot be provided."""
+    global _row_ops, _row_ops_error
+    if _row_ops is not None:
+        return _row_ops
+    if _row_ops_error is not None:
+        raise _row_ops_error
+    try:
+        lib = get_native()
+        if not row_ops_built():
+            if os.environ.get('SGV_NO_BUILD') == '1':
+                raise NativeLibraryError('%s is missing or stale and building is disabled' % ROW_OPS_PATH)
+            build_row_ops()
+        loader = importlib.machinery.ExtensionFileLoader('_sgv_row_ops', ROW_OPS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader('_sgv_row_ops', loader))
+        loader.exec_module(module)
+        module.bind([ctypes.cast(lib[name], ctypes.c_void_p).value for name in _ROW_OPS_ENTRIES])
+        _row_ops = module
+        return module
+    except Exception as exc:
+        _row_ops_error = exc if isinstance(exc, NativeLibraryError) else NativeLibraryError(str(exc))
+        raise _row_ops_error
 
 
 # ----------------------------------------------------------------------------------------------
@@ -387,11 +466,11 @@ class device_guard:
     __slots__ = ('idx', 'prev')
 
     def __init__(self, tensor):
-        self.idx = tensor.get_device()
+        self.idx = tensor.device.index
 
     def __enter__(self):
         import torch
-        self.prev = torch._C._cuda_getDevice()      # (torch.cuda.current_device() without its look at the lazy initialisation: the tensor is on a device)
+        self.prev = torch.cuda.current_device()
         if self.prev != self.idx:
             torch.cuda.set_device(self.idx)
 
@@ -400,37 +479,6 @@ class device_guard:
             import torch
             torch.cuda.set_device(self.prev)
         return False
-
-
-class PackedEntry:
-    """An entry point `int f(const block*, int dtype, void* stream)` called with the fields of its parameter block as plain values (pointers as integers, 0 for none), on
-    the current stream of a tensor's device.  For operators whose kernels take as long as their launch shim: packing the fields into bytes and passing those takes
-    0.8 us of host time, filling a ctypes.Structure and passing it 2.3 us."""
-    _CODES = {c_void_p: 'Q', c_int64: 'q', c_int32: 'i', c_float: 'f'}
-
-    def __init__(self, name, block):
-        self.name, self.block, self.fn = name, block, None
-
-    def _bind(self):
-        import torch
-        pack = struct.Struct('@' + ''.join(self._CODES[t] for _, t in self.block._fields_))
-        fields = [getattr(self.block, name) for name, _ in self.block._fields_]
-        assert pack.size <= ctypes.sizeof(self.block) < pack.size + 8 and fields[-1].offset + fields[-1].size == pack.size     # (native alignment: the compiler's, less the padding behind the last field)
-        fn = get_native()[self.name]         # a function object of its own: the shared one takes the structure
-        fn.restype, fn.argtypes = c_int, [ctypes.c_char_p, c_int, c_void_p]
-        self.pack, self.device, self.stream, self.fn = pack.pack, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, fn
-
-    def __call__(self, tensor, dtype, *fields):
-        if self.fn is None:
-            self._bind()
-        idx = tensor.get_device()
-        if self.device() == idx:
-            rc = self.fn(self.pack(*fields), dtype, self.stream(idx))
-        else:
-            with device_guard(tensor):
-                rc = self.fn(self.pack(*fields), dtype, self.stream(idx))
-        if rc:
-            check(rc)
 
 
 def launch_count():

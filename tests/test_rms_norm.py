@@ -21,14 +21,14 @@ def test_definition_and_gradient_by_differences():
     assert torch.autograd.gradcheck(lambda a: rn.rms_norm(a), (x,))
 
 
-def test_gradient_formula_is_the_derivative():
-    """The closed form that the backward pass is built on (and takes itself for second derivatives) against autograd through the definition."""
-    h, w, dy, dh = _rand(5, 33, seed=1, dtype=torch.float32).requires_grad_(True), _rand(33, seed=2, dtype=torch.float32).requires_grad_(True), _rand(5, 33, seed=3), _rand(5, 33, seed=4)
-    hd, wd = h.detach().double().requires_grad_(True), w.detach().double().requires_grad_(True)
-    want = torch.autograd.grad((rn.rms_norm_ref(hd, wd, eps=1e-3) * dy).sum() + (hd * dh).sum(), (hd, wd))
-    got = rn._gradient_ref(dy.float(), h, dh.float(), w, 1e-3)
-    for a, b in zip(got, want):
-        assert torch.allclose(a.double(), b, rtol=1e-5, atol=1e-6)      # sums of 33 (dx) and 5 (dw) fp32 terms of order 1: 40 * 2^-24 = 2.4e-6 relative to them
+def test_the_torch_side_is_built_and_takes_no_cpu_tensors():
+    ops = custom_ops.get_row_ops()
+    x, q = torch.zeros([2, 16]), torch.zeros([2, 16], dtype=torch.int8)
+    for call in (lambda: ops.rms_norm(x, None, None, 1e-8), lambda: ops.rms_norm_int8(x, None, None, 1e-8, True), lambda: ops.dequantize_rows(q, x[:, 0], 0),
+                 lambda: ops.matmul(q, x[:, 0], q, x[:, 0], None, 1, 0.0, 1.0, 0), lambda: ops.dense(x, q, x[:, 0], None, 1, 0.0, 1.0, False, 1e-8)):
+        with pytest.raises(ops.Refused):
+            call()
+    assert issubclass(ops.Refused, RuntimeError)
 
 
 def test_int8_output_on_cpu():
