@@ -189,6 +189,7 @@ _ROW_OPS_HASH_PATH = ROW_OPS_PATH + '.md5'
 _ROW_OPS_ENTRIES = ['sgv_rms_norm', 'sgv_rms_norm_backward', 'sgv_rms_norm_backward_workspace_bytes', 'sgv_dequantize_rows', 'sgv_int8_gemm', 'sgv_last_error']
 _row_ops = None
 _row_ops_error = None
+_row_ops_lock = threading.Lock()
 
 
 def row_ops_digest():
@@ -239,23 +240,26 @@ def get_row_ops():
     global _row_ops, _row_ops_error
     if _row_ops is not None:
         return _row_ops
-    if _row_ops_error is not None:
-        raise _row_ops_error
-    try:
-        lib = get_native()
-        if not row_ops_built():
-            if os.environ.get('SGV_NO_BUILD') == '1':
-                raise NativeLibraryError('%s is missing or stale and building is disabled' % ROW_OPS_PATH)
-            build_row_ops()
-        loader = importlib.machinery.ExtensionFileLoader('_sgv_row_ops', ROW_OPS_PATH)
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader('_sgv_row_ops', loader))
-        loader.exec_module(module)
-        module.bind([ctypes.cast(lib[name], ctypes.c_void_p).value for name in _ROW_OPS_ENTRIES])
-        _row_ops = module
-        return module
-    except Exception as exc:
-        _row_ops_error = exc if isinstance(exc, NativeLibraryError) else NativeLibraryError(str(exc))
-        raise _row_ops_error
+    with _row_ops_lock:
+        if _row_ops is not None:
+            return _row_ops
+        if _row_ops_error is not None:
+            raise _row_ops_error
+        try:
+            lib = get_native()
+            if not row_ops_built():
+                if os.environ.get('SGV_NO_BUILD') == '1':
+                    raise NativeLibraryError('%s is missing or stale and building is disabled' % ROW_OPS_PATH)
+                build_row_ops()
+            loader = importlib.machinery.ExtensionFileLoader('_sgv_row_ops', ROW_OPS_PATH)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader('_sgv_row_ops', loader))
+            loader.exec_module(module)
+            module.bind([ctypes.cast(lib[name], ctypes.c_void_p).value for name in _ROW_OPS_ENTRIES])
+            _row_ops = module
+            return module
+        except Exception as exc:
+            _row_ops_error = exc if isinstance(exc, NativeLibraryError) else NativeLibraryError(str(exc))
+            raise _row_ops_error
 
 
 # ----------------------------------------------------------------------------------------------

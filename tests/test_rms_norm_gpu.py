@@ -256,6 +256,57 @@ def test_refusals_on_the_gpu():
     assert de.shape == (0, 8) and not dw.any()
 
 
+def test_empty_batches_and_lost_inputs():
+    for shape in ((0, 24), (2, 0, 24), (0, 3, 24)):
+        x = torch.empty(shape, device=DEV, requires_grad=True)
+        y, h = rn.rms_norm(x, None, torch.empty(shape, device=DEV))
+        assert y.shape == h.shape == shape
+        (dx,) = torch.autograd.grad([y, h], [x], [torch.empty(shape, device=DEV)] * 2)
+        assert dx.shape == shape
+        with torch.no_grad():
+            q, s = rn.rms_norm_int8(x)
+            assert q.shape == shape and s.shape == shape[:-1] and int8.dequantize_rows(q, s).shape == shape
+            assert int8.matmul(q, s, torch.ones([5, 24], dtype=torch.int8, device=DEV), torch.ones(5, device=DEV)).shape == shape[:-1] + (5,)
+            assert int8.dense(x, torch.ones([5, 24], dtype=torch.int8, device=DEV), torch.ones(5, device=DEV), normalize=True).shape == shape[:-1] + (5,)
+    x, w = _rand(4, 24).requires_grad_(True), torch.ones(24, device=DEV, requires_grad=True)
+    y, h = rn.rms_norm(x, w, x)
+    h.add_(1)                                       # the gradient needs the stream as it was
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
+def test_two_threads_on_two_streams():
+    import threading
+    sets = [(_rand(700, 1111).requires_grad_(True), _rand(1111).requires_grad_(True), _rand(700, 1111)) for _ in range(2)]
+
+    def once(x, w, dy):
+        y = rn.rms_norm(x, w)
+        with torch.no_grad():
+            q, s = rn.rms_norm_int8(x, w)
+            p = int8.matmul(q, s, q, s)
+        return torch.autograd.grad(y, (x, w), dy) + (y.detach(), q, s, p)
+
+    want = [once(*s) for s in sets]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = once(*sets[i])
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    bad.append(i)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_streams_and_graph_replays():
     x, r, w, dy = _rand(300, 1000, seed=1), _rand(300, 1000, seed=2), _rand(1000, seed=3), _rand(300, 1000, seed=4)
     ins = [t.clone().requires_grad_(True) for t in (x, w, r)]
