@@ -15,28 +15,33 @@ struct args {
 // does fp32 hold the sum of squares?  (a sum below the range matters only where eps does not cover it)
 __device__ __forceinline__ bool sum_in_range(float ss, float eps) { return ss < 1e37f && (ss > 1e-30f || eps > 1e-20f); }
 
-// The 8-bit values of VEC columns, four to a word.  v(j): the value in steps of the row, good to 4e-5 (|v| <= 127: at most five roundings of 2^-24); u64(j): the exact u.
-// Adding 1.5 * 2^23 leaves the nearest whole number in the low bits.
-template <int VEC, typename V, typename U>
-__device__ __forceinline__ void quantise(V v, U u64, double amax, unsigned* word) {
-    constexpr float MAGIC = 12582912.f;
-    float x[VEC], far = 0.f;
+// The 8-bit values of VEC columns, four to a word.  x(j): 384 + the value in steps of the row -- between 257 and 511, where the float's last place is 2^-15 -- so that its
+// bits, shifted by one, hold the whole number in byte 2 (off by 128) and the fraction in the two bytes below: one addition rounds, and values within NEAR / 2^16 of a border
+// between two steps show in the low half.  (x is good to 3.5 / 2^16: rcp, two products and the sum of the largest at 2^-24 .. 2^-23 each, 127 times that, and half a last
+// place.)  They are decided by the exact sign of 127 u - (N - 1/2) max|u|, halves to the even neighbour; u64(j): the exact u.
+constexpr unsigned NEAR = 4;
+template <int VEC, typename X, typename U>
+__device__ __forceinline__ void quantise(X x, U u64, double amax, unsigned* word) {
+    unsigned y[VEC];
+    unsigned short near = 0xffff;
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
-        const float s = v(j);
-        x[j] = s + MAGIC;
-        far = __builtin_fmaxf(far, __builtin_fabsf(s - (x[j] - MAGIC)));
+        const float s = x(j);
+        y[j] = (__float_as_uint(s) << 1) + (0x808000u + NEAR);
+        near = min(near, (unsigned short)y[j]);
     }
-    if (far > 0.49995f) {
+    if (near < 2 * NEAR) {
 #pragma unroll
-        for (int j = 0; j < VEC; j++) x[j] = (float)__builtin_rint(u64(j) * 127.0 / amax) + MAGIC;
+        for (int j = 0; j < VEC; j++)
+            if ((unsigned short)y[j] < 2 * NEAR) {
+                const int n = (int)(y[j] << 8) >> 24;
+                const double m = (double)n - 0.5, p = amax * m, e = __builtin_fma(u64(j), 127.0, -p) - __builtin_fma(amax, m, -p);
+                if (e < 0.0 || (e == 0.0 && (n & 1))) y[j] -= 0x10000u;
+            }
     }
 #pragma unroll
-    for (int w = 0; w < VEC / 4; w++) {
-        const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(x[4 * w + 1]), __float_as_uint(x[4 * w]), 0x0c0c0400u);
-        const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(x[4 * w + 3]), __float_as_uint(x[4 * w + 2]), 0x04000c0cu);
-        word[w] = lo | hi;
-    }
+    for (int w = 0; w < VEC / 4; w++)
+        word[w] = __builtin_amdgcn_perm(y[4 * w + 1], y[4 * w], 0x0c0c0602u) | __builtin_amdgcn_perm(y[4 * w + 3], y[4 * w + 2], 0x06020c0cu);
 }
 template <int VEC>
 __device__ __forceinline__ void store_bytes(int8_t* q, const unsigned* word) {
@@ -53,6 +58,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
     __shared__ red_slots red;
     int turn = 0;
     const int t = threadIdx.x % TEAM;
+    const bool partial = p.cols % VEC != 0;
     int col[NV], shared[NV];
 #pragma unroll
     for (int v = 0; v < NV; v++) col[v] = vec_column<TEAM, VEC>(v, t, p.cols, shared[v]);
@@ -94,7 +100,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
             float part = ss;
 #pragma unroll
             for (int j = 0; j < VEC; j++) part = __builtin_fmaf(h[v][j], h[v][j], part);
-            if (shared[v] > 0) {
+            if (partial && shared[v] > 0) {
                 part = ss;
 #pragma unroll
                 for (int j = 0; j < VEC; j++) part = j >= shared[v] ? __builtin_fmaf(h[v][j], h[v][j], part) : part;
@@ -104,16 +110,15 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 float w[VEC];
                 weight.get(v, w);
                 if constexpr (WK == W_NONE) {            // a NaN does not show in this maximum, but in the sum of squares
-                    float m = __uint_as_float(top);
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) m = __builtin_fmaxf(m, __builtin_fabsf(h[v][j]));
-                    top = __float_as_uint(m);
+                    for (int j = 0; j < VEC; j += 2) top = max3_abs(top, h[v][j], h[v][j + 1]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < VEC; j++) top = max(top, abs_bits(h[v][j] * w[j]));
                 }
             }
         }
+        const unsigned mine = top;
         team_reduce<TEAM, OUT8>(ss, top, red, turn);
         float inv = 1.f;
         if (p.normalize) {
@@ -139,31 +144,34 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 put_vec<T, STREAM>((T*)p.y + row * p.cols, col[v], p.cols, io<T>::pack(y));
             }
         } else {
-            // EXACT: fp32 holds every product h * w (all there is without a weight, and products of two 16-bit values), the maximum too
+            // EXACT: fp32 holds every product h * w (all there is without a weight, and products of two 16-bit values), the maximum too.  Elsewhere the largest product is
+            // among those that round to the largest.
             constexpr bool EXACT = WK == W_NONE || (WK == W_ROWS && VEC == 8);
             const float peak = WK == W_NONE && ss != ss ? ss : __uint_as_float(top);
-            // ... unless it leaves fp32's range or comes near its end: rows of zeros are among these
-            const bool wide = !EXACT || !(peak > 1e-30f && peak < 1e37f);
+            // wide: the maximum leaves fp32's range or comes near its end (rows of zeros are among these)
+            const bool wide = !(peak > 1e-30f && peak < 1e37f);
             double amax = (double)peak, k64 = 0.0;
             bool fine = true;
             float k, scale;
-            if (wide) {
-                if (peak == peak) {
-                    double top64 = 0.0;
+            auto exact_top = [&] {
+                double top64 = 0.0;
 #pragma unroll
-                    for (int v = 0; v < NV; v++) {
-                        float w[VEC];
-                        weight.get(v, w);
+                for (int v = 0; v < NV; v++) {
+                    float w[VEC];
+                    weight.get(v, w);
 #pragma unroll
-                        for (int j = 0; j < VEC; j++) top64 = __builtin_fmax(top64, __builtin_fabs((double)h[v][j] * w[j]));
-                    }
-                    amax = team_wide<TEAM>(top64, red, turn, max_op());
+                    for (int j = 0; j < VEC; j++) top64 = __builtin_fmax(top64, __builtin_fabs((double)h[v][j] * w[j]));
                 }
+                return top64;
+            };
+            if (wide) {
+                if (peak == peak) amax = team_wide<TEAM>(exact_top(), red, turn, max_op());
                 fine = amax > 0.0 && amax < __builtin_inf();
                 scale = fine || amax == 0.0 ? (float)(amax * inv / 127.0) : __builtin_nanf("");
                 k64 = fine ? 127.0 / amax : 0.0;
                 k = 0.f;
             } else {
+                if constexpr (!EXACT) amax = team_wide<TEAM>(mine == top ? exact_top() : 0.0, red, turn, max_op());
                 k = 127.f * __builtin_amdgcn_rcpf(peak);
                 scale = peak * inv * (1.f / 127.f);
             }
@@ -178,8 +186,8 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 if (!fine) {
 #pragma unroll
                     for (int e = 0; e < VEC / 4; e++) word[e] = 0u;
-                } else if (wide) quantise<VEC>([&](int j) { return (float)(u64(j) * k64); }, u64, amax, word);
-                else quantise<VEC>([&](int j) { return h[v][j] * w[j] * k; }, u64, amax, word);
+                } else if (wide) quantise<VEC>([&](int j) { return (float)(u64(j) * k64) + 384.f; }, u64, amax, word);
+                else quantise<VEC>([&](int j) { return __builtin_fmaf(WK == W_NONE ? h[v][j] : h[v][j] * w[j], k, 384.f); }, u64, amax, word);
                 if (col[v] < p.cols) store_bytes<VEC>(q + col[v], word);
             }
             if (t < p.q_cols - p.cols) q[p.cols + t] = 0;
@@ -259,7 +267,7 @@ __global__ __launch_bounds__(TEAM) void rms_norm_long_kernel(const args p) {
                     io<T>::unpack(load_vec<T, true>(again, i, p.cols), h);
                     load_weight<T, true>(p.weight, p.weight_f32, i, p.cols, w);
                 }
-                if (fine) quantise<VEC>([&](int j) { return i + j < p.cols ? (float)((double)h[j] * w[j] * k64) : 0.f; }, [&](int j) { return i + j < p.cols ? (double)h[j] * w[j] : 0.0; }, amax, word);
+                if (fine) quantise<VEC>([&](int j) { return i + j < p.cols ? (float)((double)h[j] * w[j] * k64) + 384.f : 384.f; }, [&](int j) { return i + j < p.cols ? (double)h[j] * w[j] : 0.0; }, amax, word);
                 else {
 #pragma unroll
                     for (int e = 0; e < VEC / 4; e++) word[e] = 0u;

@@ -189,6 +189,12 @@ struct add_op { __device__ __forceinline__ double operator()(double a, double b)
 struct max_op { __device__ __forceinline__ double operator()(double a, double b) const { return a > b ? a : b; } };      // (of numbers; NaN is looked for elsewhere)
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }                       // orders magnitudes, NaN above infinity
+// the largest magnitude so far and two more values (one instruction; a NaN is passed over).  In assembly: of __builtin_fmaxf each argument is made canonical first.
+__device__ __forceinline__ unsigned max3_abs(unsigned top, float a, float b) {
+    unsigned r;
+    asm("v_max3_f32 %0, %1, |%2|, |%3|" : "=v"(r) : "v"(top), "v"(a), "v"(b));
+    return r;
+}
 
 // The vector v of thread t of a row: its first column, and how many of its columns the vector in front of it has too.  A row whose length is no multiple of VEC ends with
 // a vector that is moved back to lie inside the row: both write the same values to the columns they share, and the sums leave them out once.
