@@ -77,6 +77,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
     for (int v = 0; v < NV; v++) weight.load(p.weight, v, col[v], p.cols);
     for (; row < p.rows; row += stride) {
         if (!AHEAD) load(row);
+        weight.fresh();
         float h[NV][VEC];
 #pragma unroll
         for (int v = 0; v < NV; v++) io<T>::unpack(xv[v], h[v]);
@@ -171,7 +172,10 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 k64 = fine ? 127.0 / amax : 0.0;
                 k = 0.f;
             } else {
-                if constexpr (!EXACT) amax = team_wide<TEAM>(mine == top ? exact_top() : 0.0, red, turn, max_op());
+                if constexpr (!EXACT) {
+                    const bool any = mine == top;
+                    amax = team_top<TEAM>(any ? exact_top() : 0.0, any, red, turn);
+                }
                 k = 127.f * __builtin_amdgcn_rcpf(peak);
                 scale = peak * inv * (1.f / 127.f);
             }

@@ -185,6 +185,27 @@ __device__ __forceinline__ double team_wide(double v, red_slots& s, int& turn, F
     }
     return v;
 }
+// The maximum of v (not below zero) over the lanes where `any` -- few -- of the threads of a row
+template <int TEAM>
+__device__ __forceinline__ double team_top(double v, bool any, red_slots& s, int& turn) {
+    double m = 0.0;
+    for (uint64_t lanes = __ballot(any); lanes; lanes &= lanes - 1) {
+        const int lane = __builtin_ctzll(lanes);
+        const uint64_t b = (uint64_t)__double_as_longlong(v);
+        const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)b, lane), hi = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(b >> 32), lane);
+        const double x = __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+        m = x > m ? x : m;
+    }
+    if constexpr (TEAM > 64) {
+        if ((threadIdx.x & 63) == 0) s.wide[turn][threadIdx.x >> 6] = m;
+        __syncthreads();
+        m = s.wide[turn][0];
+#pragma unroll
+        for (int w = 1; w < TEAM / 64; w++) m = s.wide[turn][w] > m ? s.wide[turn][w] : m;
+        turn ^= 1;
+    }
+    return m;
+}
 struct add_op { __device__ __forceinline__ double operator()(double a, double b) const { return a + b; } };
 struct max_op { __device__ __forceinline__ double operator()(double a, double b) const { return a > b ? a : b; } };      // (of numbers; NaN is looked for elsewhere)
 
@@ -232,6 +253,15 @@ struct held_weight {
         if constexpr (WK == W_F32) {
             raw[v][0] = i < cols ? load_vec<float, false>((const float*)w, i, cols) : u32x4{0u, 0u, 0u, 0u};
             raw[v][1] = i < cols ? load_vec<float, false>((const float*)w, i + 4, cols) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    // once per row: keeps the compiler from holding the unpacked weight (and its fp64 form) over the rows, which takes twice the registers
+    __device__ __forceinline__ void fresh() {
+        if constexpr (WK != W_NONE) {
+#pragma unroll
+            for (int v = 0; v < NV; v++)
+#pragma unroll
+                for (int i = 0; i < (WK == W_F32 ? 2 : 1); i++) asm volatile("" : "+v"(raw[v][i]));
         }
     }
     __device__ __forceinline__ void get(int v, float* f) const {
