@@ -371,7 +371,8 @@ extern "C" int sgv_rms_norm(const sgv_rms_norm_params* q, int dtype, void* strea
     hipStream_t stream = (hipStream_t)stream_;
     const double es = (double)sgv_dtype_size(dtype), n = (double)q->rows * q->cols, bytes = n * (es * (q->residual ? 3 : 1) + (q->q ? 1.0 : es));
     p.inv_cols = (float)(1.0 / q->cols);
-    p.stream = sgv_rn::streams(bytes, dtype, q->cols, {{q->x, q->x_stride}, {q->residual, q->residual_stride}, {q->h, q->cols}, {q->y, q->cols}});
+    // (8 bits out: a call mostly reads, and gains from 320 MB: [16384, 4096] fp32 63 -> 57 us; [16384, 4096] bf16, 201 MB, 38.8 -> 39.3 with it)
+    p.stream = sgv_rn::streams(q->q ? 1.2 * bytes : bytes, dtype, q->cols, {{q->x, q->x_stride}, {q->residual, q->residual_stride}, {q->h, q->cols}, {q->y, q->cols}});
     sgv_launch_scope scope(SGV_K_RMS_NORM, stream, bytes);
     if (dtype == SGV_F32) sgv_rn::launch_forward<float>(p, stream);
     else if (dtype == SGV_F16) sgv_rn::launch_forward<sgv_half_t>(p, stream);

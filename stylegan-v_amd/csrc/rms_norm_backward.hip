@@ -15,6 +15,7 @@ template <typename T, bool STREAM, bool DW, int WK, int TEAM, int NV>
 __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_kernel(const bwd_args p) {
     constexpr int VEC = io<T>::VEC, RPB = TEAM == 64 ? 4 : 1;
     constexpr bool AHEAD = TEAM < 1024;
+    const bool partial = p.cols % VEC != 0;
     __shared__ red_slots red;
     __shared__ float part[DW && TEAM == 64 ? 3 * 64 * NV * VEC : 1];
     int turn = 0;
@@ -45,6 +46,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_ker
     }
     for (; row < p.rows; row += stride) {
         if (!AHEAD) load(row);
+        weight.fresh();
         float g[NV][VEC], xh[NV][VEC], c = 0.f;
         u32x4 e[NV];
         const float iv = inv;
@@ -64,7 +66,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_ker
             float sum = c;
 #pragma unroll
             for (int j = 0; j < VEC; j++) sum = __builtin_fmaf(g[v][j], xh[v][j], sum);
-            if (shared[v] > 0) {
+            if (partial && shared[v] > 0) {
                 sum = c;
 #pragma unroll
                 for (int j = 0; j < VEC; j++) sum = j >= shared[v] ? __builtin_fmaf(g[v][j], xh[v][j], sum) : sum;
