@@ -49,11 +49,12 @@ __device__ __forceinline__ void store_bytes(int8_t* q, const unsigned* word) {
     else ((any_u32*)q)->v = word[0];
 }
 
-// OUT8: q and its scale, else y.  TEAM threads (64: a wave, four rows per workgroup; else the workgroup) hold a row as NV vectors each and walk over rows; the next
+// OUT8: q and its scale, else y.  TEAM threads (up to 64: of a wave, 256 / TEAM rows to a workgroup; else the workgroup) hold a row as NV vectors each and walk over rows; the next
 // row's loads are in flight while one is reduced and written.
 template <typename T, bool STREAM, bool OUT8, int WK, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const args p) {
-    constexpr int VEC = io<T>::VEC, RPB = TEAM == 64 ? 4 : 1;
+__global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void rms_norm_kernel(const args p) {
+    constexpr int VEC = io<T>::VEC, RPB = TEAM <= 64 ? 256 / TEAM : 1;
+    constexpr bool TAIL = TEAM == 1;
     constexpr bool AHEAD = TEAM < 1024;              // (1024 threads have 128 registers each)
     __shared__ red_slots red;
     int turn = 0;
@@ -66,13 +67,13 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
     auto load = [&](int64_t row) {
         const T* x = (const T*)p.x + row * p.x_stride;
         const T* r = p.residual ? (const T*)p.residual + row * p.residual_stride : x;
-        load_row<T, STREAM, NV>(x, col, p.cols, xv);
-        if (p.residual) load_row<T, STREAM, NV>(r, col, p.cols, rv);
+        load_row<T, STREAM, TAIL, NV>(x, col, p.cols, xv);
+        if (p.residual) load_row<T, STREAM, TAIL, NV>(r, col, p.cols, rv);
     };
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TEAM;
     if (AHEAD && row < p.rows) load(row);
-    held_weight<T, WK, NV> weight;
+    held_weight<T, WK, TAIL, NV> weight;
 #pragma unroll
     for (int v = 0; v < NV; v++) weight.load(p.weight, v, col[v], p.cols);
     for (; row < p.rows; row += stride) {
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 for (int j = 0; j < VEC; j++) h[v][j] += rf[j];
                 const u32x4 hv = io<T>::pack(h[v]);
                 io<T>::unpack(hv, h[v]);
-                put_vec<T, STREAM>((T*)p.h + row * p.cols, col[v], p.cols, hv);
+                put_vec<T, STREAM, TAIL>((T*)p.h + row * p.cols, col[v], p.cols, hv);
             }
         }
         if (AHEAD && row + stride < p.rows) load(row + stride);
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 weight.get(v, w);
 #pragma unroll
                 for (int j = 0; j < VEC; j++) y[j] = WK == W_NONE ? h[v][j] * inv : h[v][j] * inv * w[j];
-                put_vec<T, STREAM>((T*)p.y + row * p.cols, col[v], p.cols, io<T>::pack(y));
+                put_vec<T, STREAM, TAIL>((T*)p.y + row * p.cols, col[v], p.cols, io<T>::pack(y));
             }
         } else {
             // EXACT: fp32 holds every product h * w (all there is without a weight, and products of two 16-bit values), the maximum too.  Elsewhere the largest product is
@@ -194,13 +195,12 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_kernel(const
                 else quantise<VEC>([&](int j) { return __builtin_fmaf(WK == W_NONE ? h[v][j] : h[v][j] * w[j], k, 384.f); }, u64, amax, word);
                 if (col[v] < p.cols) store_bytes<VEC>(q + col[v], word);
             }
-            if (t < p.q_cols - p.cols) q[p.cols + t] = 0;
+            for (int i = p.cols + t; i < p.q_cols; i += TEAM) q[i] = 0;
         }
     }
 }
 
-// Rows that are not held in registers -- longer than a workgroup's, or shorter than a vector (a wave's): TEAM threads walk over the row once per step.  With a residual,
-// the later walks read the h that the same thread wrote.
+// Rows longer than a workgroup holds in registers: TEAM threads walk over the row once per step.  With a residual, the later walks read the h that the same thread wrote.
 template <typename T, bool OUT8, int TEAM>
 __global__ __launch_bounds__(TEAM) void rms_norm_long_kernel(const args p) {
     constexpr int VEC = io<T>::VEC;
@@ -321,7 +321,7 @@ __global__ __launch_bounds__(256) void dequantize_rows_kernel(const int8_t* q, i
 template <typename T, bool STREAM, bool OUT8, int WK>
 struct forward_go {
     const args& p; int64_t blocks; hipStream_t stream;
-    template <int TEAM, int NV> void go() const { hipLaunchKernelGGL((rms_norm_kernel<T, STREAM, OUT8, WK, TEAM, NV>), dim3((unsigned)blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, stream, p); }
+    template <int TEAM, int NV> void go() const { hipLaunchKernelGGL((rms_norm_kernel<T, STREAM, OUT8, WK, TEAM, NV>), dim3((unsigned)blocks), dim3(TEAM <= 64 ? 256 : TEAM), 0, stream, p); }
 };
 template <typename T, bool STREAM, bool OUT8>
 static void launch_forward(const args& p, const shape& s, hipStream_t stream) {
@@ -334,8 +334,7 @@ template <typename T, bool OUT8>
 static void launch_forward(const args& p, hipStream_t stream) {
     const shape s = row_shape(p.cols, io<T>::VEC);
     const dim3 grid((unsigned)groups(p.rows, s, false));
-    if (s.elems == 0 && s.team == 64) hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT8, 64>), grid, dim3(64), 0, stream, p);
-    else if (s.elems == 0) hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT8, 1024>), grid, dim3(1024), 0, stream, p);
+    if (s.elems == 0) hipLaunchKernelGGL((rms_norm_long_kernel<T, OUT8, 1024>), grid, dim3(1024), 0, stream, p);
     else if (p.stream) launch_forward<T, true, OUT8>(p, s, stream);
     else launch_forward<T, false, OUT8>(p, s, stream);
 }

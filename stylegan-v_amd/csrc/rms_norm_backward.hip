@@ -12,12 +12,12 @@ struct bwd_args {
 };
 
 template <typename T, bool STREAM, bool DW, int WK, int TEAM, int NV>
-__global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_kernel(const bwd_args p) {
-    constexpr int VEC = io<T>::VEC, RPB = TEAM == 64 ? 4 : 1;
-    constexpr bool AHEAD = TEAM < 1024;
+__global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void rms_norm_backward_kernel(const bwd_args p) {
+    constexpr int VEC = io<T>::VEC, RPB = TEAM <= 64 ? 256 / TEAM : 1;
+    constexpr bool AHEAD = TEAM < 1024, TAIL = TEAM == 1;
     const bool partial = p.cols % VEC != 0;
     __shared__ red_slots red;
-    __shared__ float part[DW && TEAM == 64 ? 3 * 64 * NV * VEC : 1];
+    __shared__ float part[DW && TEAM <= 64 ? 3 * TEAM * NV * VEC : 1];
     int turn = 0;
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     int col[NV], shared[NV];
@@ -26,15 +26,15 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_ker
     u32x4 gv[NV], hv[NV], ev[NV];
     float inv;
     auto load = [&](int64_t row) {
-        load_row<T, STREAM, NV>((const T*)p.dy + row * p.dy_stride, col, p.cols, gv);
-        load_row<T, STREAM, NV>((const T*)p.h + row * p.h_stride, col, p.cols, hv);
-        if (p.dh) load_row<T, STREAM, NV>((const T*)p.dh + row * p.dh_stride, col, p.cols, ev);
+        load_row<T, STREAM, TAIL, NV>((const T*)p.dy + row * p.dy_stride, col, p.cols, gv);
+        load_row<T, STREAM, TAIL, NV>((const T*)p.h + row * p.h_stride, col, p.cols, hv);
+        if (p.dh) load_row<T, STREAM, TAIL, NV>((const T*)p.dh + row * p.dh_stride, col, p.cols, ev);
         inv = p.inv_rms[row];
     };
     const int64_t stride = (int64_t)gridDim.x * RPB;
     int64_t row = (int64_t)blockIdx.x * RPB + team;
     if (AHEAD && row < p.rows) load(row);
-    held_weight<T, WK, NV> weight;
+    held_weight<T, WK, TAIL, NV> weight;
 #pragma unroll
     for (int v = 0; v < NV; v++) weight.load(p.weight, v, col[v], p.cols);
     float dw[DW ? NV : 1][VEC];
@@ -85,31 +85,40 @@ __global__ __launch_bounds__(TEAM == 64 ? 256 : TEAM) void rms_norm_backward_ker
                 }
 #pragma unroll
                 for (int j = 0; j < VEC; j++) d[j] = __builtin_fmaf(iv, __builtin_fmaf(-xh[v][j], c, g[v][j]), d[j]);
-                put_vec<T, STREAM>((T*)p.dx + row * p.cols, col[v], p.cols, io<T>::pack(d));
+                put_vec<T, STREAM, TAIL>((T*)p.dx + row * p.cols, col[v], p.cols, io<T>::pack(d));
             }
         }
     }
     if constexpr (DW) {
-        if constexpr (TEAM == 64) {       // the four waves' sums, in the order of the waves
-            if (team > 0) {
+        if constexpr (TEAM <= 64) {       // the sums of a wave's rows, then those of the four waves, in the order of the waves
+            for (int off = TEAM; off < 64; off <<= 1)
 #pragma unroll
                 for (int v = 0; v < NV; v++)
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) part[((team - 1) * NV + v) * 64 * VEC + j * 64 + t] = dw[v][j];
+                    for (int j = 0; j < VEC; j++) dw[v][j] += __shfl_xor(dw[v][j], off, 64);
+            const int wave = threadIdx.x >> 6;
+            if (wave > 0 && (threadIdx.x & 63) < TEAM) {
+#pragma unroll
+                for (int v = 0; v < NV; v++)
+#pragma unroll
+                    for (int j = 0; j < VEC; j++) part[((wave - 1) * NV + v) * TEAM * VEC + j * TEAM + t] = dw[v][j];
             }
             __syncthreads();
-            if (team > 0) return;
+            if (threadIdx.x >= TEAM) return;
 #pragma unroll
             for (int w = 0; w < 3; w++)
 #pragma unroll
                 for (int v = 0; v < NV; v++)
 #pragma unroll
-                    for (int j = 0; j < VEC; j++) dw[v][j] += part[(w * NV + v) * 64 * VEC + j * 64 + t];
+                    for (int j = 0; j < VEC; j++) dw[v][j] += part[(w * NV + v) * TEAM * VEC + j * TEAM + t];
         }
         float* out = p.partials + (int64_t)blockIdx.x * p.cols;
 #pragma unroll
         for (int v = 0; v < NV; v++)
-            if (col[v] < p.cols) {
+            if (TAIL) {
+#pragma unroll
+                for (int j = 0; j < VEC; j++) if (j < p.cols) out[j] = dw[v][j];
+            } else if (col[v] < p.cols) {
 #pragma unroll
                 for (int q = 0; q < VEC / 4; q++) ((any_f32x4*)(out + col[v] + 4 * q))->v = f32x4{dw[v][4 * q], dw[v][4 * q + 1], dw[v][4 * q + 2], dw[v][4 * q + 3]};
             }
@@ -177,7 +186,7 @@ __global__ __launch_bounds__(1024) void rms_norm_weight_grad_kernel(const float*
 template <typename T, bool STREAM, bool DW, int WK>
 struct backward_go {
     const bwd_args& p; int64_t blocks; hipStream_t stream;
-    template <int TEAM, int NV> void go() const { hipLaunchKernelGGL((rms_norm_backward_kernel<T, STREAM, DW, WK, TEAM, NV>), dim3((unsigned)blocks), dim3(TEAM == 64 ? 256 : TEAM), 0, stream, p); }
+    template <int TEAM, int NV> void go() const { hipLaunchKernelGGL((rms_norm_backward_kernel<T, STREAM, DW, WK, TEAM, NV>), dim3((unsigned)blocks), dim3(TEAM <= 64 ? 256 : TEAM), 0, stream, p); }
 };
 template <typename T, bool STREAM, bool DW>
 static void launch_backward(const bwd_args& p, const shape& s, int64_t blocks, hipStream_t stream) {
@@ -187,8 +196,7 @@ static void launch_backward(const bwd_args& p, const shape& s, int64_t blocks, h
 }
 template <typename T>
 static void launch_backward(const bwd_args& p, const shape& s, int64_t blocks, hipStream_t stream) {
-    if (s.elems == 0 && s.team == 64) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T, 64>), dim3((unsigned)blocks), dim3(64), 0, stream, p);
-    else if (s.elems == 0) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T, 1024>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
+    if (s.elems == 0) hipLaunchKernelGGL((rms_norm_backward_long_kernel<T, 1024>), dim3((unsigned)blocks), dim3(1024), 0, stream, p);
     else if (p.partials) { if (p.stream) launch_backward<T, true, true>(p, s, blocks, stream); else launch_backward<T, false, true>(p, s, blocks, stream); }
     else { if (p.stream) launch_backward<T, true, false>(p, s, blocks, stream); else launch_backward<T, false, false>(p, s, blocks, stream); }
 }

@@ -7,7 +7,7 @@
 //   gradient, with g = dy * w and xh = h * inv:  dx = dr = inv * (g - xh * mean_k(g xh)) + dh,   dw = sum_rows dy * xh
 //
 // All of it is bound by memory (12 operations per element against 3..10 bytes): a row is read once into registers, 16 bytes per lane and load, at most 16 elements to a
-// thread, and nothing is read again.  Rows of up to 1024 elements are one wave's (no barrier at all), longer ones a workgroup's of 128..1024 threads; workgroups walk
+// thread, and nothing is read again.  Rows of up to 1024 elements are one wave's or share one (no barrier at all), longer ones a workgroup's of 128..1024 threads; workgroups walk
 // over rows with the next row's loads in flight while one is reduced and written, and hold the weight in registers.  Rows beyond 16384 elements are walked over
 // three times (the later reads come from the L2).  16-byte accesses need no alignment on this chip, so odd lengths and strides take the same kernels: a row's last,
 // partial vector is moved back to end with the row.  Calls that move more than the caches hold go past them.
@@ -147,10 +147,33 @@ __device__ __forceinline__ unsigned wave_max(unsigned v) {
 #undef SGV_RN_STEP
     return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
+// Rows of 8, 16 or 32 lanes, several to a wave: quad_perm 1, 2, half mirror, mirror and a swizzle; every lane ends with the same bits, sums being of equal pairs.
+__device__ __forceinline__ unsigned swap16(unsigned v) { return (unsigned)__builtin_amdgcn_ds_swizzle((int)v, 0x401f); }
+template <int TEAM> __device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (TEAM >= 8) {
+        v += __uint_as_float(dpp<0xb1, 0xf>(__float_as_uint(v)));
+        v += __uint_as_float(dpp<0x4e, 0xf>(__float_as_uint(v)));
+        v += __uint_as_float(dpp<0x141, 0xf>(__float_as_uint(v)));
+    }
+    if constexpr (TEAM >= 16) v += __uint_as_float(dpp<0x140, 0xf>(__float_as_uint(v)));
+    if constexpr (TEAM >= 32) v += __uint_as_float(swap16(__float_as_uint(v)));
+    return v;
+}
+template <int TEAM> __device__ __forceinline__ unsigned lanes_max(unsigned v) {
+    if constexpr (TEAM >= 8) { v = max(v, dpp<0xb1, 0xf>(v)); v = max(v, dpp<0x4e, 0xf>(v)); v = max(v, dpp<0x141, 0xf>(v)); }
+    if constexpr (TEAM >= 16) v = max(v, dpp<0x140, 0xf>(v));
+    if constexpr (TEAM >= 32) v = max(v, swap16(v));
+    return v;
+}
 struct red_slots { float sum[2][16]; unsigned top[2][16]; double wide[2][16]; };
 // sum and maximum of a row together (MAX false: the sum alone)
 template <int TEAM, bool MAX>
 __device__ __forceinline__ void team_reduce(float& sum, unsigned& top, red_slots& s, int& turn) {
+    if constexpr (TEAM < 64) {
+        sum = lanes_sum<TEAM>(sum);
+        if constexpr (MAX) top = lanes_max<TEAM>(top);
+        return;
+    }
     sum = wave_sum(sum);
     if constexpr (MAX) top = wave_max(top);
     if constexpr (TEAM > 64) {
@@ -174,7 +197,7 @@ __device__ __forceinline__ float team_sum(float v, red_slots& s, int& turn) {
 template <int TEAM, typename F>
 __device__ __forceinline__ double team_wide(double v, red_slots& s, int& turn, F f) {
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
+    for (int off = TEAM < 64 ? TEAM / 2 : 32; off > 0; off >>= 1) v = f(v, __shfl_xor(v, off, 64));
     if constexpr (TEAM > 64) {
         if ((threadIdx.x & 63) == 0) s.wide[turn][threadIdx.x >> 6] = v;
         __syncthreads();
@@ -185,9 +208,12 @@ __device__ __forceinline__ double team_wide(double v, red_slots& s, int& turn, F
     }
     return v;
 }
+struct add_op { __device__ __forceinline__ double operator()(double a, double b) const { return a + b; } };
+struct max_op { __device__ __forceinline__ double operator()(double a, double b) const { return a > b ? a : b; } };      // (of numbers; NaN is looked for elsewhere)
 // The maximum of v (not below zero) over the lanes where `any` -- few -- of the threads of a row
 template <int TEAM>
 __device__ __forceinline__ double team_top(double v, bool any, red_slots& s, int& turn) {
+    if constexpr (TEAM < 64) return team_wide<TEAM>(v, s, turn, max_op());
     double m = 0.0;
     for (uint64_t lanes = __ballot(any); lanes; lanes &= lanes - 1) {
         const int lane = __builtin_ctzll(lanes);
@@ -206,8 +232,6 @@ __device__ __forceinline__ double team_top(double v, bool any, red_slots& s, int
     }
     return m;
 }
-struct add_op { __device__ __forceinline__ double operator()(double a, double b) const { return a + b; } };
-struct max_op { __device__ __forceinline__ double operator()(double a, double b) const { return a > b ? a : b; } };      // (of numbers; NaN is looked for elsewhere)
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return __builtin_bit_cast(unsigned, v) & 0x7fffffffu; }                       // orders magnitudes, NaN above infinity
 // the largest magnitude so far and two more values (one instruction; a NaN is passed over).  In assembly: of __builtin_fmaxf each argument is made canonical first.
@@ -218,41 +242,42 @@ __device__ __forceinline__ unsigned max3_abs(unsigned top, float a, float b) {
 }
 
 // The vector v of thread t of a row: its first column, and how many of its columns the vector in front of it has too.  A row whose length is no multiple of VEC ends with
-// a vector that is moved back to lie inside the row: both write the same values to the columns they share, and the sums leave them out once.
+// a vector that is moved back to lie inside the row: both write the same values to the columns they share, and the sums leave them out once.  A row shorter than a vector is
+// one thread's (TEAM = 1), whose vector ends with zeros.
 template <int TEAM, int VEC>
 __device__ __forceinline__ int vec_column(int v, int t, int cols, int& shared) {
     int i = (v * TEAM + t) * VEC;
     shared = 0;
-    if (i < cols && i + VEC > cols) { shared = i + VEC - cols; i = cols - VEC; }
+    if (TEAM > 1 && i < cols && i + VEC > cols) { shared = i + VEC - cols; i = cols - VEC; }
     return i;
 }
 
-template <typename T, bool STREAM, int NV>
+template <typename T, bool STREAM, bool TAIL, int NV>
 __device__ __forceinline__ void load_row(const T* row, const int* col, int cols, u32x4* out) {
 #pragma unroll
     for (int v = 0; v < NV; v++) {
         out[v] = u32x4{0u, 0u, 0u, 0u};
-        if (col[v] < cols) out[v] = STREAM ? stream_vec(row, col[v]) : load_vec<T, false>(row, col[v], cols);
+        if (col[v] < cols) out[v] = STREAM ? stream_vec(row, col[v]) : load_vec<T, TAIL>(row, col[v], cols);
     }
 }
-template <typename T, bool STREAM>
+template <typename T, bool STREAM, bool TAIL>
 __device__ __forceinline__ void put_vec(T* row, int i, int cols, const u32x4& v) {
     if (i >= cols) return;
-    if (STREAM) stream_vec(row, i, v); else store_vec<T, false>(row, i, cols, v);
+    if (STREAM) stream_vec(row, i, v); else store_vec<T, TAIL>(row, i, cols, v);
 }
 
 // How the weight is kept: not at all, in the rows' type, in fp32 beside 16-bit rows.
 enum weight_kind { W_NONE, W_ROWS, W_F32 };
 // The weight of a thread's columns: loaded once per workgroup, kept as it is stored.
-template <typename T, int WK, int NV>
+template <typename T, int WK, bool TAIL, int NV>
 struct held_weight {
     static constexpr int VEC = io<T>::VEC;
     u32x4 raw[WK == W_NONE ? 1 : NV][WK == W_F32 ? 2 : 1];
     __device__ __forceinline__ void load(const void* w, int v, int i, int cols) {
-        if constexpr (WK == W_ROWS) raw[v][0] = i < cols ? load_vec<T, false>((const T*)w, i, cols) : u32x4{0u, 0u, 0u, 0u};
+        if constexpr (WK == W_ROWS) raw[v][0] = i < cols ? load_vec<T, TAIL>((const T*)w, i, cols) : u32x4{0u, 0u, 0u, 0u};
         if constexpr (WK == W_F32) {
-            raw[v][0] = i < cols ? load_vec<float, false>((const float*)w, i, cols) : u32x4{0u, 0u, 0u, 0u};
-            raw[v][1] = i < cols ? load_vec<float, false>((const float*)w, i + 4, cols) : u32x4{0u, 0u, 0u, 0u};
+            raw[v][0] = i < cols ? load_vec<float, TAIL>((const float*)w, i, cols) : u32x4{0u, 0u, 0u, 0u};
+            raw[v][1] = i < cols ? load_vec<float, TAIL>((const float*)w, i + 4, cols) : u32x4{0u, 0u, 0u, 0u};
         }
     }
     // once per row: keeps the compiler from holding the unpacked weight (and its fp64 form) over the rows, which takes twice the registers
@@ -274,12 +299,13 @@ struct held_weight {
     }
 };
 
-// How a row is held: TEAM threads with at most 16 elements each, or not at all (elems = 0, the walking kernels: one wave for rows shorter than a vector, 1024 threads for
-// rows beyond 16384 elements)
+// How a row is held: TEAM threads with at most 16 elements each, or not at all (elems = 0, the walking kernels: 1024 threads for rows beyond 16384 elements).  Rows of
+// up to 64 vectors have as many lanes as vectors, up to a power of two ([262144, 128] bf16: a wave to a row 34 us forward, 53 to 8 bits, 102 backward with the weight's
+// gradient; 16 lanes 20.5, 20 and 41), rows shorter than a vector one ([1000000, 5] bf16: a wave 593 us forward, 5.0 ms backward; a thread 11 and 21 us).
 struct shape { int team, elems; };
 static inline shape row_shape(int cols, int vec) {
-    static const shape held[] = {{64, 4}, {64, 8}, {64, 16}, {128, 16}, {256, 16}, {512, 16}, {1024, 16}};
-    if (cols < vec) return shape{64, 0};
+    static const shape held[] = {{8, 4}, {16, 4}, {32, 4}, {64, 4}, {8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}, {128, 16}, {256, 16}, {512, 16}, {1024, 16}};
+    if (cols < vec) return shape{1, vec};
     for (const shape& s : held) if (s.elems >= vec && cols <= s.team * s.elems) return s;
     return shape{1024, 0};
 }
@@ -290,10 +316,9 @@ constexpr int MAX_COLS = (1 << 26) - 1;          // (the launch that adds up the
 // [4096, 16384] 102, 110, 124), four to a CU of 128 threads ([30000, 1111] fp16: 74 us, two 84, one 113), two of four short rows ([65536, 512] bf16: 52 us, one 62,
 // four 57); four rows to each at least ([2049, 1111] fp16: 13.4 us with two).
 static inline int64_t groups(int64_t rows, const shape& s, bool dw) {
-    const bool four = s.team == 64 && s.elems > 0;       // four rows to a workgroup
-    const int64_t teams = four ? (rows + 3) / 4 : rows;
-    const int threads = four ? 256 : s.team;
-    const int64_t most = dw ? std::min<int64_t>(four ? 512 : threads <= 128 ? 1024 : 256, std::max<int64_t>(256, rows / 4)) : 512 * (2048 / threads);
+    const int threads = std::max(s.team, 256 * (s.team <= 64)), rpb = threads / s.team;
+    const int64_t teams = (rows + rpb - 1) / rpb;
+    const int64_t most = dw ? std::min<int64_t>(rpb > 1 ? 512 : threads <= 128 ? 1024 : 256, std::max<int64_t>(256, rows / 4)) : 512 * (2048 / threads);
     return std::min(teams, most);
 }
 
@@ -301,7 +326,11 @@ static inline int64_t groups(int64_t rows, const shape& s, bool dw) {
 template <typename T, typename F>
 static void for_shape(const shape& s, F f) {
     constexpr int VEC = io<T>::VEC;
-    if (s.team == 64) {
+    if (s.team == 1) f.template go<1, 1>();
+    else if (s.team == 8) f.template go<8, 1>();
+    else if (s.team == 16) f.template go<16, 1>();
+    else if (s.team == 32) f.template go<32, 1>();
+    else if (s.team == 64) {
         if constexpr (VEC == 4) { if (s.elems == 4) { f.template go<64, 1>(); return; } }
         if (s.elems == 8) f.template go<64, 8 / VEC>(); else f.template go<64, 16 / VEC>();
     } else if (s.team == 128) f.template go<128, 16 / VEC>();
