@@ -7,18 +7,18 @@
 //   gradient, with g = dy * w and xh = h * inv:  dx = dr = inv * (g - xh * mean_k(g xh)) + dh,   dw = sum_rows dy * xh
 //
 // All of it is bound by memory (12 operations per element against 3..10 bytes): a row is read once into registers, 16 bytes per lane and load, at most 16 elements to a
-// thread, and nothing is read again.  Rows of up to 1024 elements are one wave's or share one (no barrier at all), longer ones a workgroup's of 128..1024 threads; workgroups walk
-// over rows with the next row's loads in flight while one is reduced and written, and hold the weight in registers.  Rows beyond 16384 elements are walked over
-// three times (the later reads come from the L2).  16-byte accesses need no alignment on this chip, so odd lengths and strides take the same kernels: a row's last,
+// thread, and nothing is read again.  Rows of up to 1024 elements are one wave's or share one (no barrier at all), longer ones a workgroup's of 128..1024 threads;
+// workgroups walk over rows with the next row's loads in flight while one is reduced and written, and hold the weight in registers.  Rows beyond 16384 elements are walked
+// over three times (the later reads come from the L2).  16-byte accesses need no alignment on this chip, so odd lengths and strides take the same kernels: a row's last,
 // partial vector is moved back to end with the row.  Calls that move more than the caches hold go past them.
-// Measured (a 1 GB copy: 5.2 TB/s): [16384, 4096] bf16 forward 42 us = 6.3 TB/s, with a residual 93 us = 5.8, to 8 bits with a residual 76 us = 6.2, backward with all
-// gradients 93 us = 5.8; [30000, 1111] fp16 forward 23 us = 5.7, backward 71 us = 3.7 (rows off the cache lines).  Rows to 8 bits without a residual are the exception:
-// 16-bit rows run at 3.8..4.3 TB/s, bound by the instructions of the rounding.
+// Measured (a 1 GB copy: 5.2 TB/s): [16384, 4096] bf16 forward 42 us = 6.4 TB/s, with a residual 93 us = 5.8, to 8 bits 39 us = 5.2 (half of it instructions: 16 an
+// element), with a residual 76 us = 6.2, backward with all gradients 90 us = 5.9; [30000, 1111] fp16 forward 23 us = 5.7, backward with all gradients 74 us = 3.6 (rows off
+// the cache lines, eleven of 128 threads with a second vector).
 //
 // Statistics are fp32: a lane sums at most 16 squares before the tree (fp64 in the walking kernels).  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a
-// tiny eps) is summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 4e-5 of a step, so a value within 5e-5 of a border
-// between two steps is decided by the fp64 quotient; the row maximum is exact because the product of two 16-bit values is exact in fp32, and other products are
-// taken in fp64.
+// tiny eps) is summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 5.4e-5 of a step, so a value within 6e-5 of a border
+// between two steps is decided in fp64; the row maximum is exact because the product of two 16-bit values is exact in fp32, and other products are taken in fp64 by the
+// lanes that hold the maximum.
 #pragma once
 
 #include "sgv_common.h"
