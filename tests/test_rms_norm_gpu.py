@@ -14,7 +14,7 @@ DEV = 'cuda'
 U = 2.0 ** -24
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 # both sides of every border of the dispatch: one thread, 8, 16, 32 lanes, one wave x 1, 2, 4 vectors, a workgroup x 2, 4, 8, the walking kernel; whole vectors and not
-LENGTHS = [1, 3, 4, 7, 8, 15, 16, 31, 32, 33, 64, 65, 120, 128, 129, 255, 256, 257, 511, 512, 513, 1024, 1025, 1111, 2048, 2049, 4096, 4100, 8192, 8193, 16384, 16385, 40001]
+LENGTHS = [1, 3, 4, 7, 8, 15, 16, 31, 32, 33, 64, 65, 120, 128, 129, 255, 256, 257, 511, 512, 513, 1024, 1025, 1111, 2048, 2049, 2900, 4096, 4100, 5121, 8192, 8193, 9000, 13313, 16384, 16385, 40001]
 
 
 def _rand(*shape, seed=0, dtype=torch.float32, scale=1.0):
