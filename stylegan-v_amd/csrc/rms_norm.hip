@@ -24,10 +24,12 @@ template <int VEC, typename X, typename U>
 __device__ __forceinline__ void quantise(X x, U u64, double amax, unsigned* word) {
     unsigned y[VEC];
     unsigned short near = 0xffff;
+    unsigned half = 0x808000u + NEAR;
+    asm("" : "+s"(half));                 // (in a register: the shift and the addition are one instruction then, which takes no literal)
 #pragma unroll
     for (int j = 0; j < VEC; j++) {
         const float s = x(j);
-        y[j] = (__float_as_uint(s) << 1) + (0x808000u + NEAR);
+        y[j] = (__float_as_uint(s) << 1) + half;
         near = min(near, (unsigned short)y[j]);
     }
     if (near < 2 * NEAR) {
