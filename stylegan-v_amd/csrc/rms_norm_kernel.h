@@ -311,14 +311,15 @@ static inline shape row_shape(int cols, int vec) {
 }
 constexpr int MAX_COLS = (1 << 26) - 1;          // (the launch that adds up the weight gradient has 64 threads for a column)
 
-// Workgroups of a launch: twice as many as the CUs hold at once (2048 threads each), which walk over the rows.  With a weight gradient they are the rows of its partial
-// sums, which should stay small beside the rows: one to a CU where a row takes 256 threads or more ([16384, 4096] bf16 with all gradients 89 us, two 94, four 108;
+// Workgroups of a launch, which walk over the rows: twice as many as 2048 threads to a CU, where rows are short; as many as the registers let a CU hold, 1024 threads, where
+// a row takes 512 threads or more ([4096, 16384] bf16 forward 41.5 us, four times as many 43.7; to 8 bits with a weight 44.4 and 49.5).  With a weight gradient they are the
+// rows of its partial sums, which should stay small beside the rows: one to a CU where a row takes 256 threads or more ([16384, 4096] bf16 with all gradients 89 us, two 94, four 108;
 // [4096, 16384] 102, 110, 124), four to a CU of 128 threads ([30000, 1111] fp16: 74 us, two 84, one 113), two of four short rows ([65536, 512] bf16: 52 us, one 62,
 // four 57); four rows to each at least ([2049, 1111] fp16: 13.4 us with two).
 static inline int64_t groups(int64_t rows, const shape& s, bool dw) {
     const int threads = std::max(s.team, 256 * (s.team <= 64)), rpb = threads / s.team;
     const int64_t teams = (rows + rpb - 1) / rpb;
-    const int64_t most = dw ? std::min<int64_t>(rpb > 1 ? 512 : threads <= 128 ? 1024 : 256, std::max<int64_t>(256, rows / 4)) : 512 * (2048 / threads);
+    const int64_t most = dw ? std::min<int64_t>(rpb > 1 ? 512 : threads <= 128 ? 1024 : 256, std::max<int64_t>(256, rows / 4)) : threads >= 512 ? 262144 / threads : 512 * (2048 / threads);
     return std::min(teams, most);
 }
 
