@@ -186,7 +186,7 @@ def emit(out):
 
 TIMED_FAMILIES = ('conv3x3_s1', 'upfirdn2d_lanes')      # kernel families whose launches are bracketed by HIP events inside the timed region (eager headline)
 CAPTURED_FAMILIES = ('conv3x3_s1',)                     # captured headline: the family whose kernel writes its own timestamps inside the replayed graphs
-PMC_FILES = ['r06_pmc_bench_step_FETCH_WRITE.json']   # collected by tools/gpu_recipes/r06_final.sh (separate --pmc passes of this command), stamped with the kernel sources' digest
+PMC_FILES = ['pmc_bench_step_FETCH_WRITE.json']   # collected as in tools/gpu_recipes/r06_final.sh (separate --pmc passes of this command), stamped with the kernel sources' digest
 
 
 PMC_NOT_THIS_WORKLOAD = None      # set when the run is not the workload the committed counter passes were collected on
