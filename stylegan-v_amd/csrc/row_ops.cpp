@@ -2,7 +2,7 @@
 // sgv_int8_gemm (include/sgv_ops.h) on the current stream of the tensors' device.
 //
 // In C++ because at a token or a small batch these operators take less time on the GPU than Python takes to call them: per call of host time, [32, 512] fp32 norm 11.3 -> 6 us
-// under autograd, forward and backward 75 -> 46 us (of which 30 are the hand-over to the autograd engine's device thread and back, where a Python backward also starts cold).
+// under autograd, forward and backward 75 -> 43 us (of which 30 are the hand-over to the autograd engine's device thread and back, where a Python backward also starts cold).
 //
 // Arguments are checked here with one predicate for each operator; `Refused` sends the caller (ops/rms_norm.py, ops/int8.py) to the check that words the reason.
 #include <ATen/ATen.h>

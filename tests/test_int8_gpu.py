@@ -132,6 +132,19 @@ def test_refusals_on_the_gpu():
     for bad in ((a.cpu(), sa, b, sb), (a, sa.cpu(), b, sb), (a, sa, b.cpu(), sb), (a, sa, b, sb.cpu())):
         with pytest.raises(RuntimeError, match='device'):
             int8.matmul(*bad)
+    g = sb.clone().requires_grad_(True)
+    for what, kw in (('activation', dict(act='relu')), ('dtype', dict(dtype=torch.float64)), ('bias', dict(bias=torch.ones(4, device=DEV))), ('bias', dict(bias=torch.ones(5)))):
+        with pytest.raises(RuntimeError, match=what):
+            int8.matmul(a, sa, b, sb, **kw)
+    x = torch.ones([4, 64], device=DEV)
+    for what, call in (('no gradient', lambda: int8.matmul(a, sa, b, g)), ('no gradient', lambda: int8.dense(x.clone().requires_grad_(True), b, sb)),
+                       ('no gradient', lambda: int8.quantize_rows(x.clone().requires_grad_(True))), ('no gradient', lambda: int8.dequantize_rows(a, sa.clone().requires_grad_(True))),
+                       ('dtype', lambda: int8.quantize_rows(x.double())), ('dtype', lambda: int8.dense(x.double(), b, sb)), ('dtype', lambda: int8.dequantize_rows(a, sa, torch.float64)),
+                       ('eps', lambda: int8.dense(x, b, sb, normalize=True, eps=-1.0)), ('eps', lambda: rn.rms_norm_int8(x, eps=float('nan'))), ('K of a', lambda: int8.dense(x[:, :60], b, sb)),
+                       ('131071', lambda: int8.matmul(*[torch.zeros([1, 131072], dtype=torch.int8, device=DEV), torch.ones(1, device=DEV)] * 2)),
+                       ('int8 rows', lambda: int8.dequantize_rows(x, sa)), ('int8 rows', lambda: int8.matmul(x, sa, b, sb))):
+        with pytest.raises(RuntimeError, match=what):
+            call()
     with pytest.raises(RuntimeError, match='device'):
         int8.matmul(a, sa, b, sb, bias=torch.zeros(5))
 
