@@ -4,7 +4,8 @@
 // In C++ because at a token or a small batch these operators take less time on the GPU than Python takes to call them: per call of host time, [32, 512] fp32 norm 11.3 -> 6 us
 // under autograd, forward and backward 75 -> 43 us (of which 30 are the hand-over to the autograd engine's device thread and back, where a Python backward also starts cold).
 //
-// Arguments are checked here with one predicate for each operator; `Refused` sends the caller (ops/rms_norm.py, ops/int8.py) to the check that words the reason.
+// Arguments are checked here with one predicate for each operator; `Refused` sends the caller (ops/rms_norm.py, ops/int8.py) to the check that words the reason, `Watched` to
+// the formula in torch operations, or to a refusal where the operator has no gradient.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -23,6 +24,7 @@ using at::Tensor;
 using std::optional;
 
 struct Refused : std::runtime_error { using std::runtime_error::runtime_error; };
+struct Watched : Refused { using Refused::Refused; };
 
 // the C entry points, as addresses in the loaded libsgv_hip.so
 struct {
@@ -50,6 +52,21 @@ void check(int rc) {
 void require(bool ok, const char* what) {
     if (!ok) throw Refused(what);
 }
+
+// Whether something follows this tensor that sees torch's operations and no launch: a derivative of forward mode by the tangent it has (a launch's output would come without
+// one, and without an error), a function transform or a subclass, whose tensors have no memory of their own.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool without_memory(const Tensor& t) {
+    using Key = c10::DispatchKey;
+    return t.defined() && t.key_set().has_any(c10::DispatchKeySet({Key::Batched, Key::FuncTorchBatched, Key::FuncTorchGradWrapper, Key::Functionalize, Key::Python, Key::ZeroTensor}));
+}
+bool has_tangent(const optional<Tensor>& t) { return t && has_tangent(*t); }
+bool without_memory(const optional<Tensor>& t) { return t && without_memory(*t); }
+template <typename... Ts> void unwatched(const Ts&... ts) {
+    if ((has_tangent(ts) || ...)) throw Watched("serves inference and has no gradient, of forward mode neither: call it with detached tensors");
+    if ((without_memory(ts) || ...)) throw Watched("takes tensors in memory: it has no form under a function transform (vmap, grad, jvp) or for a tensor subclass");
+}
+template <typename... Ts> bool watched(const Ts&... ts) { return ((has_tangent(ts) || without_memory(ts)) || ...); }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
@@ -148,7 +165,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
         Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor(), dx, dw;
         const bool need_w = (needs & 2) && dy.defined();
         if (!dy.defined() && !dh.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-        if (at::GradMode::is_enabled()) {
+        if (at::GradMode::is_enabled() || watched(dy, dh, h, weight)) {
             std::tie(dx, dw) = gradient_formula(dy, h, dh, weight, ctx->saved_data["eps"].toDouble());
         } else if (!dy.defined()) {
             dx = dh;
@@ -182,6 +199,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 };
 
 std::tuple<Tensor, optional<Tensor>> rms_norm(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual, double eps) {
+    unwatched(x, weight, residual);
     require(rows_fit(x, weight, residual, eps), "rms_norm: arguments");
     const Tensor rows = row_view(x);
     const optional<Tensor> res = residual ? optional<Tensor>(row_view(*residual)) : optional<Tensor>();
@@ -203,6 +221,7 @@ std::tuple<Tensor, optional<Tensor>> rms_norm(const Tensor& x, const optional<Te
 }
 
 std::tuple<Tensor, Tensor, optional<Tensor>> rms_norm_int8(const Tensor& x, const optional<Tensor>& weight, const optional<Tensor>& residual, double eps, bool normalize) {
+    unwatched(x, weight, residual);
     require(rows_fit(x, weight, residual, eps) && !(at::GradMode::is_enabled() && (x.requires_grad() || wants_grad(weight) || wants_grad(residual))), "rms_norm_int8: arguments");
     Forward out = launch_forward(row_view(x), dense_or_none(weight), residual ? row_view(*residual) : Tensor(), eps, true, normalize, false);
     if (x.dim() != 2) {
@@ -215,6 +234,7 @@ std::tuple<Tensor, Tensor, optional<Tensor>> rms_norm_int8(const Tensor& x, cons
 }
 
 Tensor dequantize_rows(const Tensor& q, const Tensor& scale, int64_t code) {
+    unwatched(q, scale);
     require(scaled_rows_fit(q, scale) && q.size(-1) <= std::numeric_limits<int32_t>::max() && !(at::GradMode::is_enabled() && scale.requires_grad()), "dequantize_rows: arguments");
     const Tensor out = at::empty(q.sizes(), q.options().dtype(code_type(code)).memory_format(at::MemoryFormat::Contiguous)), rows = row_view(q), s = dense_or_none(scale);
     if (rows.size(0)) {
@@ -265,6 +285,7 @@ at::DimVector layer_shape(const Tensor& x, const Tensor& b) {
 
 Tensor matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale, const optional<Tensor>& bias, int act, double alpha, double gain, int64_t code) {
     const Epilogue e{bias, act, alpha, gain};
+    unwatched(a, a_scale, b, b_scale, bias);
     require(scaled_rows_fit(a, a_scale) && layer_fits(a.size(-1), a.device(), b, b_scale, e) && !(at::GradMode::is_enabled() && a_scale.requires_grad()), "matmul: arguments");
     const Tensor out = at::empty(layer_shape(a, b), a.options().dtype(code_type(code)));
     if (out.numel()) {
@@ -276,6 +297,7 @@ Tensor matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Ten
 
 Tensor dense(const Tensor& x, const Tensor& b, const Tensor& b_scale, const optional<Tensor>& bias, int act, double alpha, double gain, bool normalize, double eps) {
     const Epilogue e{bias, act, alpha, gain};
+    unwatched(x, b, b_scale, bias);
     require(rows_fit(x, {}, {}, eps) && layer_fits(x.size(-1), x.device(), b, b_scale, e) && !(at::GradMode::is_enabled() && x.requires_grad()), "dense: arguments");
     const Tensor out = at::empty(layer_shape(x, b), x.options());
     if (out.numel()) {
@@ -289,6 +311,7 @@ Tensor dense(const Tensor& x, const Tensor& b, const Tensor& b_scale, const opti
 
 PYBIND11_MODULE(_sgv_row_ops, m) {
     pybind11::register_exception<Refused>(m, "Refused", PyExc_RuntimeError);
+    pybind11::register_exception<Watched>(m, "Watched", m.attr("Refused"));
     const pybind11::call_guard<pybind11::gil_scoped_release> no_gil;       // (a launch waits where the queue is full)
     m.def("bind", &bind);
     m.def("rms_norm", &rms_norm, no_gil);

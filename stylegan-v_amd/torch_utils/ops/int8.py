@@ -34,6 +34,8 @@ def dequantize_rows(q, scale, dtype=torch.float32):
         ops = custom_ops.get_row_ops()
         try:
             return ops.dequantize_rows(q, scale, _rn._DTYPE_CODES[dtype])
+        except ops.Watched as seen:
+            raise RuntimeError(f'dequantize_rows {seen}') from None
         except (ops.Refused, TypeError, KeyError):
             _check_dequantize(q, scale, dtype)
             raise
@@ -93,6 +95,8 @@ def matmul(a, a_scale, b, b_scale, bias=None, act='linear', act_gain=None, dtype
         try:
             kind, alpha, gain = _acts[act]
             return ops.matmul(a, a_scale, b, b_scale, bias, kind, alpha, gain if act_gain is None else act_gain, _rn._DTYPE_CODES[dtype])
+        except ops.Watched as seen:
+            raise RuntimeError(f'matmul {seen}') from None
         except (ops.Refused, TypeError, KeyError):
             _check_matmul(a, a_scale, b, b_scale, bias, dtype, act)
             raise
@@ -108,6 +112,8 @@ def dense(x, weight, weight_scale, bias=None, act='linear', act_gain=None, norma
         try:
             kind, alpha, gain = _acts[act]
             return ops.dense(x, weight, weight_scale, bias, kind, alpha, gain if act_gain is None else act_gain, normalize, eps)
+        except ops.Watched as seen:
+            raise RuntimeError(f'dense {seen}') from None
         except (ops.Refused, TypeError, KeyError):
             _rn._check('dense', x, None, None, eps)
             _check_layer('dense', x.shape[-1], x.device, weight, weight_scale, bias, x.dtype, act)

@@ -7,7 +7,8 @@ a gradient of its own:
     y = h * rsqrt(mean(h^2) + eps) * weight
 
 One launch forward and one backward (two with a weight, whose gradient is a sum over all rows; its order is fixed, so equal inputs give equal bits).  A gradient that is
-itself differentiated (``create_graph``) takes the same formula as a composition of torch ops.
+itself differentiated (``create_graph``) takes the same formula as a composition of torch ops, and so do both directions under derivatives of forward mode and function
+transforms (``torch.func``).
 
 ``rms_norm_int8`` gives y in 8 bits with one scale per row -- the left operand of ``ops.int8.matmul`` -- in the same single pass: y is never written in its own type.
 It serves inference and has no gradient.
@@ -15,6 +16,7 @@ It serves inference and has no gradient.
 Statistics are fp32 whatever the rows' type (fp32, fp16, bf16).  CPU tensors take the plain torch formulation.
 """
 import torch
+import torch.autograd.forward_ad as _fwd
 
 from .. import custom_ops
 
@@ -22,10 +24,13 @@ _DTYPE_CODES = {torch.float32: custom_ops.SGV_F32, torch.float16: custom_ops.SGV
 
 
 def check_no_grad(what, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f'{what} serves inference and has no gradient: call it under torch.no_grad() or with detached tensors')
+    for t in tensors:
+        if t is None:
+            continue
+        if torch.is_grad_enabled() and t.requires_grad:
+            raise RuntimeError(f'{what} serves inference and has no gradient: call it under torch.no_grad() or with detached tensors')
+        if _fwd.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f'{what} serves inference and has no gradient, of forward mode neither: call it with detached tensors')
 
 
 def _check(what, x, weight, residual, eps):
@@ -65,6 +70,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-8):
         ops = custom_ops.get_row_ops()
         try:
             out = ops.rms_norm(x, weight, residual, eps)
+        except ops.Watched:
+            _check('rms_norm', x, weight, residual, eps)
+            return rms_norm_ref(x, weight, residual, eps)
         except (ops.Refused, TypeError):
             _check('rms_norm', x, weight, residual, eps)
             raise
@@ -103,6 +111,8 @@ def launch_int8(what, x, weight, residual, eps, normalize):
     ops = custom_ops.get_row_ops()
     try:
         return ops.rms_norm_int8(x, weight, residual, eps, normalize)
+    except ops.Watched as seen:
+        raise RuntimeError(f'{what} {seen}') from None
     except (ops.Refused, TypeError):
         _check(what, x, weight, residual, eps)
         check_no_grad(what, x, weight, residual)
