@@ -8,8 +8,10 @@
 // the formula in torch operations, or to a refusal where the operator has no gradient.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/sgv_ops.h"
@@ -54,7 +56,8 @@ void require(bool ok, const char* what) {
 }
 
 // Whether something follows this tensor that sees torch's operations and no launch: a derivative of forward mode by the tangent it has (a launch's output would come without
-// one, and without an error), a function transform or a subclass, whose tensors have no memory of their own.
+// one, and without an error), a function transform or a subclass, whose tensors have no memory of their own; or whether torch records a graph of its operations, which would
+// hold the outputs' allocation and not what fills them (torch.jit.trace, make_fx).
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
 bool without_memory(const Tensor& t) {
     using Key = c10::DispatchKey;
@@ -62,11 +65,16 @@ bool without_memory(const Tensor& t) {
 }
 bool has_tangent(const optional<Tensor>& t) { return t && has_tangent(*t); }
 bool without_memory(const optional<Tensor>& t) { return t && without_memory(*t); }
+bool recorded() {
+    return torch::jit::tracer::isTracing() ||
+           (c10::impl::TorchDispatchModeTLS::any_modes_set() && c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value());
+}
 template <typename... Ts> void unwatched(const Ts&... ts) {
+    if (recorded()) throw Watched("launches a kernel, which a trace does not record: trace the function without it, or the layer before quantize_int8_()");
     if ((has_tangent(ts) || ...)) throw Watched("serves inference and has no gradient, of forward mode neither: call it with detached tensors");
     if ((without_memory(ts) || ...)) throw Watched("takes tensors in memory: it has no form under a function transform (vmap, grad, jvp) or for a tensor subclass");
 }
-template <typename... Ts> bool watched(const Ts&... ts) { return ((has_tangent(ts) || without_memory(ts)) || ...); }
+template <typename... Ts> bool watched(const Ts&... ts) { return recorded() || ((has_tangent(ts) || without_memory(ts)) || ...); }
 
 void* stream_of(const Tensor& t) { return (void*)c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 

@@ -6,7 +6,8 @@
 
 A weight is quantised once (``quantize_rows(weight)``: one scale per output channel), activations at every call (one scale per token).  The sums are exact 32-bit integers,
 so a result depends neither on how the product is split nor on the other rows of a batch; scales, bias and activation are applied in fp32, rounded once to the output's type.
-All of it serves inference and has no gradient.  CPU tensors take the plain torch formulation.
+All of it serves inference and has no gradient.  CPU tensors take the plain torch formulation.  On the GPU a call is a launch that torch's tracers and function transforms
+would not see: it refuses them.
 """
 import torch
 

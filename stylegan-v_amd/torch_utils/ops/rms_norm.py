@@ -7,8 +7,8 @@ a gradient of its own:
     y = h * rsqrt(mean(h^2) + eps) * weight
 
 One launch forward and one backward (two with a weight, whose gradient is a sum over all rows; its order is fixed, so equal inputs give equal bits).  A gradient that is
-itself differentiated (``create_graph``) takes the same formula as a composition of torch ops, and so do both directions under derivatives of forward mode and function
-transforms (``torch.func``).
+itself differentiated (``create_graph``) takes the same formula as a composition of torch ops, and so do both directions under derivatives of forward mode, function
+transforms (``torch.func``) and while a graph of torch's operations is recorded (``torch.jit.trace``, ``make_fx``).
 
 ``rms_norm_int8`` gives y in 8 bits with one scale per row -- the left operand of ``ops.int8.matmul`` -- in the same single pass: y is never written in its own type.
 It serves inference and has no gradient.
