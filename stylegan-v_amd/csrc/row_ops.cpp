@@ -135,11 +135,12 @@ Forward launch_forward(const Tensor& x, const Tensor& weight, const Tensor& resi
     return out;
 }
 
-// (dx, dweight) in torch operations: what the kernel computes, differentiable once more
+// (dx, dweight) in torch operations: what the kernel computes, differentiable once more.  The norm is fp64, as the kernel's is where squares leave fp32's range; the
+// normalised row, of sqrt(columns) at most, is fp32 again.
 std::tuple<Tensor, Tensor> gradient_formula(const Tensor& dy, const Tensor& h, const Tensor& dh, const Tensor& weight, double eps) {
     Tensor dx, dw;
     if (dy.defined()) {
-        const Tensor hf = h.to(at::kFloat), inv = (hf.square().mean(-1, true) + eps).rsqrt(), xh = hf * inv;
+        const Tensor hd = h.to(at::kDouble), inv = (hd.square().mean(-1, true) + eps).rsqrt(), xh = (hd * inv).to(at::kFloat);
         Tensor g = dy.to(at::kFloat);
         if (weight.defined()) {
             dw = (g * xh).sum(0).to(weight.scalar_type());

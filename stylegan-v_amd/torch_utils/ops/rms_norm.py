@@ -55,9 +55,11 @@ def _wide(t):
 
 
 def rms_norm_ref(x, weight=None, residual=None, eps=1e-8):
-    """The definition, in torch ops."""
+    """The definition, in torch ops.  The norm is fp64: squares of what fp32 and bf16 hold leave fp32's range."""
     h = x if residual is None else (_wide(x) + _wide(residual)).to(x.dtype)
-    y = _wide(h) * (_wide(h).square().mean(dim=-1, keepdim=True) + eps).rsqrt()
+    hd = h.double()
+    y = hd * (hd.square().mean(dim=-1, keepdim=True) + eps).rsqrt()
+    y = y if x.dtype == torch.float64 else y.float()
     if weight is not None:
         y = y * _wide(weight)
     y = y.to(x.dtype)

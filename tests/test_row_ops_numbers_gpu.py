@@ -1,0 +1,46 @@
+"""Row norm on the GPU at the ends of fp32's range: the forms of a value that are not a launch of the kernel alone."""
+import pytest
+import torch
+
+from stylegan_v_amd.torch_utils.ops import rms_norm as rn
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+U = 2.0 ** -24
+
+
+def _rand(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(list(shape), generator=torch.Generator().manual_seed(seed), dtype=torch.float64).to(dtype).to(DEV)
+
+
+def _formula(x, w, r, eps):
+    h = x + r
+    return h * (h.square().mean(dim=-1, keepdim=True) + eps).rsqrt() * w, h
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('scale', [1e30, 1e20, 1.0, 1e-25])
+def test_second_derivative_of_rows_out_of_range(dtype, scale):
+    """The gradient under create_graph is the first-order kernel's, and its own gradient the formula's, whatever the rows' size."""
+    eps = 0.0
+    ins = [(_rand(4, 50, seed=1) * scale).to(dtype), _rand(50, seed=2, dtype=dtype), (_rand(4, 50, seed=3) * scale).to(dtype)]
+    dy = _rand(4, 50, seed=4, dtype=dtype)
+    a = [t.clone().requires_grad_(True) for t in ins]
+    first = torch.autograd.grad(rn.rms_norm(*a, eps=eps)[0], a, dy)
+    b = [t.clone().requires_grad_(True) for t in ins]
+    under = torch.autograd.grad(rn.rms_norm(*b, eps=eps)[0], b, dy, create_graph=True)
+    # both forms are within 200 U of the exact gradient's terms, whose size is at most a few times the largest of a row's; and each is rounded once to the type
+    for got, want in zip(under, first):
+        assert torch.isfinite(got).all() and want.any()
+        assert (got.double() - want.double()).abs().max() <= (2000 * U + 2 * torch.finfo(dtype).eps) * want.double().abs().max()
+    v = _rand(50, seed=5, dtype=dtype)
+    (second,) = torch.autograd.grad(under[1], b[0], v)
+    # the same in 64 bits, on the stream as it was rounded
+    h64 = (ins[0].double() + ins[2].double()).to(dtype).double().requires_grad_(True)
+    w64 = ins[1].double().requires_grad_(True)
+    y64, _ = _formula(h64, w64, torch.zeros_like(h64), eps)
+    (gw,) = torch.autograd.grad(y64, w64, dy.double(), create_graph=True)
+    (want,) = torch.autograd.grad(gw, h64, v.double())
+    assert torch.isfinite(second).all()
+    top = torch.finfo(dtype).smallest_normal           # (1e30: the second derivative is 1e-30 and below)
+    assert (second.double() - want).abs().max() <= (2000 * U + 4 * torch.finfo(dtype).eps) * want.abs().max() + top
