@@ -86,14 +86,19 @@ at::ScalarType code_type(int64_t code) {
     return code == SGV_F32 ? at::kFloat : code == SGV_F16 ? at::kHalf : at::kBFloat16;
 }
 
-// t as [rows, columns] with unit stride along a row: a view where t allows one, else a copy
+// t as [rows, columns] with unit stride along a row: a view where t allows one, else a copy.  (A negated view, whose memory holds the values with the other sign, is copied:
+// so are dense_or_none's and the gradients that arrive.)
 Tensor row_view(const Tensor& t) {
+    if (t.is_neg()) return row_view(t.resolve_neg());
     const int64_t cols = t.size(-1);
     if (t.is_contiguous()) return t.dim() == 2 ? t : t.view({-1, cols});
     Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
     return cols > 1 && r.stride(1) != 1 ? r.contiguous() : r;
 }
-Tensor dense_or_none(const Tensor& t) { return !t.defined() || t.is_contiguous() ? t : t.contiguous(); }
+Tensor dense_or_none(const Tensor& t) {
+    if (!t.defined() || (t.is_contiguous() && !t.is_neg())) return t;
+    return t.resolve_neg().contiguous();
+}
 Tensor dense_or_none(const optional<Tensor>& t) { return t ? dense_or_none(*t) : Tensor(); }
 const void* ptr(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
 void* out_ptr(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -180,6 +185,8 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
             dx = dh;
         } else {
             const int64_t rows = h.size(0), cols = h.size(1);
+            if (dy.is_neg()) dy = dy.resolve_neg();
+            if (dh.defined() && dh.is_neg()) dh = dh.resolve_neg();
             if (cols > 1 && dy.stride(1) != 1) dy = dy.contiguous();
             if (cols > 1 && dh.defined() && dh.stride(1) != 1) dh = dh.contiguous();
             const Tensor w = dense_or_none(weight);
