@@ -28,8 +28,10 @@ class FullyConnectedLayer(torch.nn.Module):
     """Equalised-learning-rate dense layer: weight stored as randn/lr_mul, used as W*lr_mul/sqrt(in)."""
 
     # (weight rows, their scales, bias, state of the parameters, their storage) of quantize_int8_: derived from the parameters, neither buffers nor state.  On the class, so
-    # that layers unpickled from before the attribute existed have it too
+    # that layers unpickled from before the attribute existed have it too.  A copy or a snapshot of a layer that serves holds `_requantise` in its place: the state is that of
+    # addresses and counters of this process, and another one may come to the same
     _int8 = None
+    _requantise = (None, None, None, None, None)
 
     def __init__(self, in_features, out_features, bias=True, activation='linear', lr_multiplier=1, bias_init=0):
         super().__init__()
@@ -46,7 +48,7 @@ class FullyConnectedLayer(torch.nn.Module):
         """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
         quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters changed or moved
         since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``, a new ``.data``) refuses to serve until it is quantised again, and so does a copy
-        of the layer.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place writes under inference mode) are not seen, and a captured
+        of the layer or one loaded from a snapshot, neither of which holds the rows.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place writes under inference mode) are not seen, and a captured
         graph keeps the weight it was captured with.  Returns the layer."""
         if self.activation not in ('linear', 'lrelu'):
             raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
@@ -56,6 +58,16 @@ class FullyConnectedLayer(torch.nn.Module):
         held = [p.detach() for p in (self.weight, self.bias) if p is not None]       # (as long as they live, no other tensor gets the addresses in the state)
         self._int8 = (rows, scales, bias, self._parameter_state(), held)
         return self
+
+    @classmethod
+    def _without_rows(cls, state):
+        return {**state, '_int8': cls._requantise} if state.get('_int8') is not None else state
+
+    def __getstate__(self):
+        return self._without_rows(super().__getstate__())
+
+    def __setstate__(self, state):
+        super().__setstate__(self._without_rows(state))
 
     def serves_int8(self):
         return self._int8 is not None and not torch.is_grad_enabled()
@@ -67,7 +79,7 @@ class FullyConnectedLayer(torch.nn.Module):
         if self.serves_int8():
             rows, scales, bias, state, _ = self._int8
             if state != self._parameter_state():
-                raise RuntimeError('the parameters of this layer changed after quantize_int8_(): quantise it again')
+                raise RuntimeError('the parameters of this layer changed after quantize_int8_(), or it is a copy: quantise it again')
             act_gain = None if gain is None else float(bias_act.activation_funcs[self.activation].def_gain * gain)
             if normalize_input and x.ndim != 2:
                 x, normalize_input = normalize_2nd_moment(x), False      # (over dimension 1, whatever the shape)
