@@ -48,8 +48,8 @@ class FullyConnectedLayer(torch.nn.Module):
         """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
         quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters changed or moved
         since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``, a new ``.data``) refuses to serve until it is quantised again, and so does a copy
-        of the layer or one loaded from a snapshot, neither of which holds the rows.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place writes under inference mode) are not seen, and a captured
-        graph keeps the weight it was captured with.  Returns the layer."""
+        of the layer or one loaded from a snapshot, neither of which holds the rows.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place
+        writes under inference mode) are not seen, and a captured graph keeps the weight it was captured with.  ``drop_int8_()`` is the way back.  Returns the layer."""
         if self.activation not in ('linear', 'lrelu'):
             raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
         with torch.no_grad():
@@ -57,6 +57,11 @@ class FullyConnectedLayer(torch.nn.Module):
             bias = self.bias.detach().float() * self.bias_gain if self.bias is not None else None
         held = [p.detach() for p in (self.weight, self.bias) if p is not None]       # (as long as they live, no other tensor gets the addresses in the state)
         self._int8 = (rows, scales, bias, self._parameter_state(), held)
+        return self
+
+    def drop_int8_(self):
+        """Serve this layer in fp32 again (also one that refuses because its parameters changed).  Returns the layer."""
+        self._int8 = None
         return self
 
     @classmethod
@@ -131,6 +136,13 @@ class MappingNetwork(torch.nn.Module):
         for module in self.modules():
             if isinstance(module, FullyConnectedLayer):
                 module.quantize_int8_()
+        return self
+
+    def drop_int8_(self):
+        """Serve the network's dense layers in fp32 again."""
+        for module in self.modules():
+            if isinstance(module, FullyConnectedLayer):
+                module.drop_int8_()
         return self
 
     def forward(self, z, c, truncation_psi=1, truncation_cutoff=None, skip_w_avg_update=False):

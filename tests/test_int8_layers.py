@@ -76,3 +76,20 @@ def test_layers_that_never_served_copy_as_before():
         assert twin._int8 is None and '_int8' not in twin.__dict__
         with torch.no_grad():
             assert torch.equal(twin(x), layer(x))
+
+
+def test_the_way_back_to_fp32():
+    layer, x = _layer(), torch.randn([5, 64])
+    with torch.no_grad():
+        want = layer(x)
+        assert not torch.equal(layer.quantize_int8_()(x), want)
+        assert layer.drop_int8_() is layer and torch.equal(layer(x), want) and not layer.serves_int8()
+        layer.quantize_int8_().weight.add_(0.5)              # one that would refuse
+        assert torch.equal(layer.drop_int8_()(x), _fp32(layer)(x))
+        twin = copy.deepcopy(layer.quantize_int8_())
+        assert torch.equal(twin.drop_int8_()(x), _fp32(layer)(x))
+        net = MappingNetwork(z_dim=32, c_dim=3, w_dim=32, num_ws=4, num_layers=2).eval()
+        z, c = torch.randn([16, 32]), torch.randn([16, 3])
+        want = net(z, c)
+        assert not torch.equal(net.quantize_int8_()(z, c), want)
+        assert net.drop_int8_() is net and torch.equal(net(z, c), want)
