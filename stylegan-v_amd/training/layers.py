@@ -44,14 +44,18 @@ class FullyConnectedLayer(torch.nn.Module):
     def _parameter_state(self):
         return tuple((p.device, p.dtype, p.data_ptr(), None if p.is_inference() else p._version) for p in (self.weight, self.bias) if p is not None) + (amax.replay_epoch(),)
 
+    def check_int8(self):
+        """Raises where the layer has no 8-bit form."""
+        if self.activation not in ('linear', 'lrelu'):
+            raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
+
     def quantize_int8_(self):
         """Serve this layer in 8-bit integers: its weight is quantised once, with one scale per output channel, and from here on every call under ``torch.no_grad()``
         quantises its input rows and multiplies in 8 bits (ops/int8.py).  Calls with gradients enabled keep the fp32 layer.  A layer whose parameters changed or moved
         since (an optimiser step, a replayed training graph, ``load_state_dict``, ``.to``, a new ``.data``) refuses to serve until it is quantised again, and so does a copy
         of the layer or one loaded from a snapshot, neither of which holds the rows.  Writes that bypass the version counters (``p.data.copy_``, kernels of one's own, in-place
         writes under inference mode) are not seen, and a captured graph keeps the weight it was captured with.  ``drop_int8_()`` is the way back.  Returns the layer."""
-        if self.activation not in ('linear', 'lrelu'):
-            raise RuntimeError(f'quantize_int8_: a layer with activation {self.activation} has no 8-bit form')
+        self.check_int8()
         with torch.no_grad():
             rows, scales = int8.quantize_rows(self.weight.detach().float() * self.weight_gain)
             bias = self.bias.detach().float() * self.bias_gain if self.bias is not None else None
@@ -133,9 +137,11 @@ class MappingNetwork(torch.nn.Module):
     def quantize_int8_(self):
         """Serve the network's dense layers in 8-bit integers (``FullyConnectedLayer.quantize_int8_``): under ``torch.no_grad()`` an unconditional network is one norm +
         quantisation, one product per layer and one quantisation between two layers.  For a generator that serves: ``G_ema.mapping.quantize_int8_()``."""
-        for module in self.modules():
-            if isinstance(module, FullyConnectedLayer):
-                module.quantize_int8_()
+        layers = [module for module in self.modules() if isinstance(module, FullyConnectedLayer)]
+        for layer in layers:
+            layer.check_int8()
+        for layer in layers:
+            layer.quantize_int8_()
         return self
 
     def drop_int8_(self):

@@ -93,3 +93,13 @@ def test_the_way_back_to_fp32():
         want = net(z, c)
         assert not torch.equal(net.quantize_int8_()(z, c), want)
         assert net.drop_int8_() is net and torch.equal(net(z, c), want)
+
+
+def test_a_network_is_quantised_whole_or_not_at_all():
+    net = MappingNetwork(z_dim=32, c_dim=3, w_dim=32, num_ws=4, num_layers=2, activation='tanh').eval()      # (its embedding is linear)
+    z, c = torch.randn([16, 32]), torch.randn([16, 3])
+    with torch.no_grad():
+        want = net(z, c)
+        with pytest.raises(RuntimeError, match='tanh'):
+            net.quantize_int8_()
+        assert torch.equal(net(z, c), want) and net.embed._int8 is None
