@@ -153,8 +153,8 @@ __global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void rms_norm_kernel(const
             // among those that round to the largest.
             constexpr bool EXACT = WK == W_NONE || (WK == W_ROWS && VEC == 8);
             const float peak = WK == W_NONE && ss != ss ? ss : __uint_as_float(top);
-            // wide: the maximum leaves fp32's range or comes near its end (rows of zeros are among these)
-            const bool wide = !(peak > 1e-30f && peak < 1e37f);
+            // wide: the maximum, or that of y, leaves fp32's range or comes near its end (rows of zeros are among these)
+            const bool wide = !(peak > 1e-30f && peak < 1e37f && peak * inv < 1e38f);
             double amax = (double)peak, k64 = 0.0;
             bool fine = true;
             float k, scale;

@@ -44,3 +44,17 @@ def test_second_derivative_of_rows_out_of_range(dtype, scale):
     assert torch.isfinite(second).all()
     top = torch.finfo(dtype).smallest_normal           # (1e30: the second derivative is 1e-30 and below)
     assert (second.double() - want).abs().max() <= (2000 * U + 4 * torch.finfo(dtype).eps) * want.abs().max() + top
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('cols', [40, 4096, 16384, 20000])
+def test_scale_near_the_end_of_the_range(dtype, cols):
+    """max |y| beyond fp32's end, a 127th of it inside: the scale is a number, whatever |h w| is."""
+    x = torch.zeros([3, cols], device=DEV)
+    x[0, 1], x[1, 2], x[2, 3] = 0.5, 1e-3, 1e6
+    x = x.to(dtype)
+    w = torch.full([cols], 1.0 / cols ** 0.5, device=DEV, dtype=torch.float64).mul(2e39).clamp(max=3e38).to(dtype)
+    q, s = rn.rms_norm_int8(x, w, eps=0.0)
+    want = (w.double().max() * cols ** 0.5 / 127).item()            # y = sqrt(cols) w at the only element of a row
+    assert want < 3.4e38 and ((s.double() - want).abs() <= 60 * U * want).all(), (s.tolist(), want)
+    assert torch.equal(q.double(), 127.0 * (x != 0))
