@@ -170,19 +170,24 @@ __global__ __launch_bounds__(TEAM) void rms_norm_backward_long_kernel(const bwd_
     }
 }
 
-// dw[k] = sum of the workgroups' partial rows: 16 columns per workgroup, 64 threads to a column (a wave adds up a column in the end); the order is fixed, so the result is too
+// dw[k] = sum of the workgroups' partial rows: 16 columns per workgroup at a time, 64 threads to a column (a wave adds up a column in the end); the order is fixed, so the
+// result is too.  A workgroup walks over columns only where a launch of one to every 16 would have 2^32 threads.
+constexpr int DW_GROUPS = 1 << 21;
 template <typename W>
 __global__ __launch_bounds__(1024) void rms_norm_weight_grad_kernel(const float* partials, int count, int cols, W* dw) {
     __shared__ float part[64][17];
-    const int c = threadIdx.x & 15, g = threadIdx.x >> 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 16;
-    const float* p = partials + min(col + c, cols - 1);
-    float s = 0.f;
+    const int c = threadIdx.x & 15, g = threadIdx.x >> 4, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int col = blockIdx.x * 16; col < cols; col += DW_GROUPS * 16) {
+        if (col >= DW_GROUPS * 16) __syncthreads();            // (the sums of the columns before have been read)
+        const float* p = partials + min(col + c, cols - 1);
+        float s = 0.f;
 #pragma unroll 8
-    for (int r = g; r < count; r += 64) s += p[(int64_t)r * cols];
-    part[g][c] = s;
-    __syncthreads();
-    s = wave_sum(part[lane][wave]);
-    if (lane == 0 && col + wave < cols) sgv_traits<W>::store(dw + col + wave, s);
+        for (int r = g; r < count; r += 64) s += p[(int64_t)r * cols];
+        part[g][c] = s;
+        __syncthreads();
+        s = wave_sum(part[lane][wave]);
+        if (lane == 0 && col + wave < cols) sgv_traits<W>::store(dw + col + wave, s);
+    }
 }
 
 template <typename T, bool STREAM, bool DW, int WK>
@@ -236,7 +241,7 @@ extern "C" int sgv_rms_norm_backward(const sgv_rms_norm_backward_params* q, int 
     else sgv_rn::launch_backward<sgv_bf16_t>(p, shape, blocks, stream);
     int rc = sgv_check_launch("rms_norm_backward_kernel");
     if (rc != SGV_OK || !q->dweight) return rc;
-    const dim3 grid((unsigned)((q->cols + 15) / 16));
+    const dim3 grid((unsigned)std::min((q->cols + 15) / 16, sgv_rn::DW_GROUPS));
     const float* part = (const float*)q->workspace;
     if (dtype == SGV_F32 || q->weight_f32) hipLaunchKernelGGL((sgv_rn::rms_norm_weight_grad_kernel<float>), grid, dim3(1024), 0, stream, part, (int)blocks, q->cols, (float*)q->dweight);
     else if (dtype == SGV_F16) hipLaunchKernelGGL((sgv_rn::rms_norm_weight_grad_kernel<sgv_half_t>), grid, dim3(1024), 0, stream, part, (int)blocks, q->cols, (sgv_half_t*)q->dweight);

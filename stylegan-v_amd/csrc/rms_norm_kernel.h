@@ -309,7 +309,7 @@ static inline shape row_shape(int cols, int vec) {
     for (const shape& s : held) if (s.elems >= vec && cols <= s.team * s.elems) return s;
     return shape{1024, 0};
 }
-constexpr int MAX_COLS = (1 << 26) - 1;          // (the launch that adds up the weight gradient has 64 threads for a column)
+constexpr int MAX_COLS = (1 << 26) - 1;
 
 // Workgroups of a launch, which walk over the rows: twice as many as 2048 threads to a CU, where rows are short; as many as the registers let a CU hold, 1024 threads, where
 // a row takes 512 threads or more ([4096, 16384] bf16 forward 41.5 us, four times as many 43.7; to 8 bits with a weight 44.4 and 49.5).  With a weight gradient they are the

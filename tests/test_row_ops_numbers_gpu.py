@@ -7,6 +7,7 @@ from stylegan_v_amd.torch_utils.ops import rms_norm as rn
 pytestmark = pytest.mark.gpu
 DEV = 'cuda'
 U = 2.0 ** -24
+EPS = 1e-6
 
 
 def _rand(*shape, seed=0, dtype=torch.float32):
@@ -58,3 +59,20 @@ def test_scale_near_the_end_of_the_range(dtype, cols):
     want = (w.double().max() * cols ** 0.5 / 127).item()            # y = sqrt(cols) w at the only element of a row
     assert want < 3.4e38 and ((s.double() - want).abs() <= 60 * U * want).all(), (s.tolist(), want)
     assert torch.equal(q.double(), 127.0 * (x != 0))
+
+
+@pytest.mark.parametrize('cols', [(1 << 25) + 40, (1 << 26) - 16, (1 << 26) - 15, (1 << 26) - 1])
+def test_weight_gradient_of_the_longest_rows(cols):
+    """Up to the longest rows there are, 2^26 - 1: a thread of a launch for each 64th of a column would be 2^32 of them, one more than a launch may have."""
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip('needs 20 GB of device memory')
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    x, dy = [torch.empty([2, cols], dtype=torch.float16, device=DEV).normal_(generator=g) for _ in range(2)]
+    w = torch.ones([cols], dtype=torch.float16, device=DEV).requires_grad_(True)
+    (dw,) = torch.autograd.grad(rn.rms_norm(x, w, eps=EPS), [w], dy)
+    inv = (x.double().square().mean(dim=1, keepdim=True) + EPS).rsqrt()
+    for part in (slice(0, 1 << 20), slice(1 << 25, (1 << 25) + (1 << 20)), slice(cols - (1 << 20), cols)):
+        t = dy[:, part].double() * x[:, part].double() * inv
+        want, size = t.sum(dim=0), t.abs().sum(dim=0)
+        # 1 / rms within 44 U, three roundings of each product, one of the sum; half a step of fp16
+        assert ((dw[part].double() - want).abs() <= 48 * U * size + 2.0 ** -11 * want.abs() * 1.0001 + 2.0 ** -24).all()
