@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
 //   many                  10007 x 512 x 512         38.6         11.7         9.2     13.9
 //                          4096 x 4096 x 4096         -          114          76       61
 //                          8192 x 8192 x 8192         -          861         581      470      (2,340 TOP/s)
-enum form { ROWS11, ROWS21, ROWS22, TILE64, TILE128, TILE256 };
+enum form { ROWS11, ROWS21, ROWS22, TILE64, TILE128, TILE256 };      // (in the order of their names in SGV_VARIANTS)
 
 static inline int64_t tiles(int m, int n, int em, int en) { return ((int64_t)(m + em - 1) / em) * ((n + en - 1) / en); }
 
@@ -397,6 +397,7 @@ extern "C" int sgv_int8_gemm(const sgv_int8_gemm_params* q, int dtype, void* str
     hipStream_t stream = (hipStream_t)stream_;
     const double m = q->m, n = q->n, k = q->k;
     sgv_launch_scope scope(SGV_K_INT8_GEMM, stream, m * k + n * k + m * n * (double)sgv_dtype_size(dtype), 2.0 * m * n * k);
+    sgv_note_variant(SGV_V_int8_rows_16x16 + f);
     if (dtype == SGV_F32) sgv_i8::launch<float>(p, f, stream);
     else if (dtype == SGV_F16) sgv_i8::launch<sgv_half_t>(p, f, stream);
     else sgv_i8::launch<sgv_bf16_t>(p, f, stream);

@@ -376,6 +376,8 @@ extern "C" int sgv_rms_norm(const sgv_rms_norm_params* q, int dtype, void* strea
     // (8 bits out: a call mostly reads, and gains from 320 MB: [16384, 4096] fp32 63 -> 57 us; [16384, 4096] bf16, 201 MB, 38.8 -> 39.3 with it)
     p.stream = sgv_rn::streams(q->q ? 1.2 * bytes : bytes, dtype, q->cols, {{q->x, q->x_stride}, {q->residual, q->residual_stride}, {q->h, q->cols}, {q->y, q->cols}});
     sgv_launch_scope scope(SGV_K_RMS_NORM, stream, bytes);
+    const bool held = sgv_rn::row_shape(q->cols, dtype == SGV_F32 ? 4 : 8).elems > 0;
+    sgv_note_variant(!held ? SGV_V_rms_norm_walked : p.stream ? SGV_V_rms_norm_held_past_caches : SGV_V_rms_norm_held);
     if (dtype == SGV_F32) sgv_rn::launch_forward<float>(p, stream);
     else if (dtype == SGV_F16) sgv_rn::launch_forward<sgv_half_t>(p, stream);
     else sgv_rn::launch_forward<sgv_bf16_t>(p, stream);

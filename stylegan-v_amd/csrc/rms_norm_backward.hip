@@ -236,6 +236,7 @@ extern "C" int sgv_rms_norm_backward(const sgv_rms_norm_backward_params* q, int 
     p.inv_cols = (float)(1.0 / q->cols);
     p.stream = sgv_rn::streams(n * es * (q->dh ? 4 : 3), dtype, q->cols, {{q->dy, q->dy_stride}, {q->h, q->h_stride}, {q->dh, q->dh_stride}, {q->dx, q->cols}});
     sgv_launch_scope scope(SGV_K_RMS_NORM, stream, n * es * (q->dh ? 4 : 3));
+    sgv_note_variant(shape.elems == 0 ? SGV_V_rms_norm_backward_walked : p.stream ? SGV_V_rms_norm_backward_held_past_caches : SGV_V_rms_norm_backward_held);
     if (dtype == SGV_F32) sgv_rn::launch_backward<float>(p, shape, blocks, stream);
     else if (dtype == SGV_F16) sgv_rn::launch_backward<sgv_half_t>(p, shape, blocks, stream);
     else sgv_rn::launch_backward<sgv_bf16_t>(p, shape, blocks, stream);
