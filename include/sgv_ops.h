@@ -542,7 +542,7 @@ int sgv_multi_scale_f32(const float* const* src, float* const* dst, const int64_
  *   h = T(x + residual)   (h = x without a residual; T: rounding to the rows' type -- the norm sees the h that is written)
  *   y = h * rsqrt(mean_k h^2 + eps) * weight
  *   8 bits:  q = 127 h weight / max_k |h weight| rounded to nearest even (exactly: decided in fp64 next to a border), q_scale = max_k |y| / 127;
- *            a row of zeros has scale 0; a row with a NaN or an infinity in y has scale NaN and zeros
+ *            a row of zeros has scale 0 (under eps = 0, where its y is NaN, NaN); a row with a NaN or an infinity in y has scale NaN and zeros
  * normalize = 0 (8-bit output only): y = h * weight -- the plain quantisation of rows.
  * Rows are fp32, fp16 or bf16 (`dtype`) with unit stride along a row; x_stride / residual_stride: elements between rows (0: one row for all); y and h are dense.
  * Rows of q start on 16 bytes; columns from `cols` up to the next multiple of 16 are written with zeros.
@@ -631,7 +631,7 @@ int sgv_prof_resume(void);
 /* Bracket only the launches of the families whose bit (1 << enum sgv_kernel_family) is set; 0 = all (the default).  bench.py times the dominant kernels inside
  * its timed region with two families enabled (two events per launch of 554 launches per iteration cost 1.4 % of the step) and the full table in a pass of its own. */
 int sgv_prof_families(uint64_t mask);
-int sgv_prof_collect(sgv_prof_entry* out /* [SGV_K_COUNT] */); /* syncs events, resets pool */
+int sgv_prof_collect(sgv_prof_entry* out /* [SGV_K_COUNT] */); /* syncs events, resets pool; writes the families of THIS header: a host built with fewer is built again */
 /* The same, launch by launch (in launch order) instead of summed per family: fills at most `max_records` entries, returns the number of recorded
  * launches (which may exceed max_records), or a negative SGV_ERR_* code.  Resets the pool like sgv_prof_collect. */
 typedef struct sgv_prof_record {

@@ -6,9 +6,9 @@
 // (row = lane & 15, bytes 16 (lane >> 4) ..+15 of 64).  The integer sums are exact whatever their order, so K is split freely over the waves of a workgroup, and the result
 // depends neither on the split nor on the other rows of a batch.
 //
-// Two kernels: int8_rows_kernel for few rows (bound by reading B once: 1 x 8192 x 8192 12.7 us = 5.3 TB/s) and few tiles, int8_tile_kernel for the rest (bound by the matrix
-// pipe's power: 8192^3 464 us = 2,370 TOP/s at 1.5 GHz, where the chip holds 2.4 GHz without load; 0.63 of the issue slots).  The table at choose() below has
-// both sides of every border.
+// Two kernels: int8_rows_kernel for few rows (bound by reading B once: 1 x 8192 x 8192 12.3 us = 5.4 TB/s) and few tiles, int8_tile_kernel for the rest (bound by the matrix
+// pipe and its power: 8192^3 takes 750 to 800 thousand clocks, 0.65 to 0.70 of the issue slots busy; 413 us = 2,660 TOP/s on a cool chip at 1.85 GHz, 490 us = 2,240 where
+// ten launches in a row have brought it down to 1.53 GHz, 420 us in the long run).  The table at choose() below has both sides of every border.
 #include "sgv_common.h"
 
 #include <algorithm>
@@ -51,8 +51,8 @@ __device__ __forceinline__ float finish(const args& p, int acc, float sa, float 
 // Tiles of C.  K is walked in stages of 128 bytes per row -- a cache line -- that go from memory straight into LDS (buffer_load ... lds: no registers, no instructions
 // to store them), S stages in a ring.  A stage's 16-byte chunks lie at position chunk ^ ((row >> 1) & 7) of their row, which makes the fragment reads below free of
 // bank conflicts.  A wave holds the fragments of one step of 64 k in registers and replaces each as soon as its last product is issued, so that the matrix pipe finds
-// the next step's fragments there; one barrier per stage.  (16x16x64 rather than 32x32x32 products: half the accumulator traffic for the same work, 557 -> 527 us at
-// 8192^3, where time is energy.  128 bytes of K per stage rather than 64: whole cache lines, 500 -> 477 us.)  Rows beyond the matrix and bytes beyond its end are outside the buffers' bounds and read as zero.
+// the next step's fragments there; one barrier per stage.  (16x16x64 rather than 32x32x32 products: half the accumulator traffic for the same work, 5 % of the time at
+// 8192^3, where time is energy.  128 bytes of K per stage rather than 64: whole cache lines, another 5 %.)  Rows beyond the matrix and bytes beyond its end are outside the buffers' bounds and read as zero.
 
 __device__ __forceinline__ i32x4 make_rsrc(const void* base, int64_t bytes) {
     const uint64_t b = (uint64_t)base;
@@ -67,7 +67,7 @@ __device__ __forceinline__ void dma16(i32x4 rsrc, unsigned lds, unsigned voff, i
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // Few tiles: every wave of a workgroup computes the whole 16 MT x 16 NT tile over its own stages of K (128 bytes per row; wave w takes stages w, w + waves, ...), in a
 // ring of S stages of LDS of its own -- no barrier in the loop --, and the waves' sums meet in LDS.  Through LDS because the matrix instruction wants 16 rows side by side:
-// read straight into registers, 16 neighbouring lanes touch 16 cache lines, and a CU gets 16 bytes a clock instead of 64 (32 x 512 x 8192: 13.0 us against 5.9).
+// read straight into registers, 16 neighbouring lanes touch 16 cache lines, and a CU gets 16 bytes a clock instead of 64 (32 x 512 x 8192: 13.0 us against 5.6).
 template <typename T, int MT, int NT, int S>
 __global__ __launch_bounds__(512) void int8_rows_kernel(const args p) {
     extern __shared__ __attribute__((aligned(128))) int8_t ring[];          // [waves][S][(MT + NT) * 16 rows][128], then [waves][MT * NT * 256] sums
@@ -318,17 +318,17 @@ __global__ __launch_bounds__(64 * WGM * WGN) void int8_tile_kernel(const args p)
 // ---------------------------------------------------------------------------------------------------------------------------------------
 // Which form serves a product (microseconds in a replayed graph, operands rotating through 3 sets, bf16 out):
 //                            m x n x k           rows kernel   64^2 tiles   128^2    256^2
-//   few rows                 32 x 512 x 8192         5.9           -          -        -        16 x 8192 x 8192: 13.2 (5.1 TB/s), 1 x 8192 x 8192: 12.7 (5.3 TB/s)
-//   few tiles, a long k     100 x 512 x 2048         4.9          6.2         9.4     24.5
-//                           512 x 512 x 2048         5.3          6.5         9.5     24.3
-//   ... a short k           256 x 512 x 512          4.1          4.0         5.3     12.0
-//   some tiles              777 x 1001 x 1030       14.3          5.8         8.0     20.0
-//                           128 x 4096 x 4096       13.4         10.2        22.4     41.3
-//   about a tile per CU    1500 x 1500 x 1500       37.3         14.1        13.6     27.2
-//                          2048 x 2048 x 2048       65.3         18.9        15.1     26.6
-//   many                  10007 x 512 x 512         38.6         11.7         9.2     13.9
-//                          4096 x 4096 x 4096         -          114          76       61
-//                          8192 x 8192 x 8192         -          861         581      470      (2,340 TOP/s)
+//   few rows                 32 x 512 x 8192         5.6           -          -        -        16 x 8192 x 8192: 13.4 (5.1 TB/s), 1 x 8192 x 8192: 12.3 (5.4 TB/s)
+//   few tiles, a long k     100 x 512 x 2048         4.7          6.2         9.1     24.3
+//                           512 x 512 x 2048         4.9          6.4         9.3     24.1
+//   ... a short k           256 x 512 x 512          4.0          3.7         5.1     11.7
+//   some tiles              777 x 1001 x 1030       14.0          5.4         8.0     19.7
+//                           128 x 4096 x 4096       13.1          9.9        22.3     41.2
+//   about a tile per CU    1500 x 1500 x 1500       37.1         13.4        13.3     27.1
+//                          2048 x 2048 x 2048       65.3         17.5        14.6     26.2
+//   many                  10007 x 512 x 512         38.4         11.4         8.8     13.7
+//                          4096 x 4096 x 4096         -          106          69       56
+//                          8192 x 8192 x 8192         -          850         535      420      (2,615 TOP/s)
 enum form { ROWS11, ROWS21, ROWS22, TILE64, TILE128, TILE256 };      // (in the order of their names in SGV_VARIANTS)
 
 static inline int64_t tiles(int m, int n, int em, int en) { return ((int64_t)(m + em - 1) / em) * ((n + en - 1) / en); }

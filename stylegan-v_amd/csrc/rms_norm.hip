@@ -57,7 +57,7 @@ template <typename T, bool STREAM, bool OUT8, int WK, int TEAM, int NV>
 __global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void rms_norm_kernel(const args p) {
     constexpr int VEC = io<T>::VEC, RPB = TEAM <= 64 ? 256 / TEAM : 1;
     constexpr bool TAIL = TEAM == 1;
-    // (1024 threads have 128 registers each: rows in flight beside fp32 rows with a weight spill, [4096, 16384] to 8 bits 87 -> 98 us; bf16 without one 63 -> 54)
+    // (1024 threads have 128 registers each: rows in flight beside fp32 rows with a weight spill, [4096, 16384] to 8 bits 82 -> 86 us; bf16 without one 60 -> 49)
     constexpr bool AHEAD = TEAM < 1024 || VEC == 8 || !OUT8 || WK == W_NONE;
     __shared__ red_slots red;
     int turn = 0;
@@ -373,7 +373,7 @@ extern "C" int sgv_rms_norm(const sgv_rms_norm_params* q, int dtype, void* strea
     hipStream_t stream = (hipStream_t)stream_;
     const double es = (double)sgv_dtype_size(dtype), n = (double)q->rows * q->cols, bytes = n * (es * (q->residual ? 3 : 1) + (q->q ? 1.0 : es));
     p.inv_cols = (float)(1.0 / q->cols);
-    // (8 bits out: a call mostly reads, and gains from 320 MB: [16384, 4096] fp32 63 -> 57 us; [16384, 4096] bf16, 201 MB, 38.8 -> 39.3 with it)
+    // (8 bits out: a call mostly reads, and gains from 320 MB: [16384, 4096] fp32 62 -> 56 us; [16384, 4096] bf16, 201 MB, 38.2 -> 38.8 with it)
     p.stream = sgv_rn::streams(q->q ? 1.2 * bytes : bytes, dtype, q->cols, {{q->x, q->x_stride}, {q->residual, q->residual_stride}, {q->h, q->cols}, {q->y, q->cols}});
     sgv_launch_scope scope(SGV_K_RMS_NORM, stream, bytes);
     const bool held = sgv_rn::row_shape(q->cols, dtype == SGV_F32 ? 4 : 8).elems > 0;
@@ -392,11 +392,11 @@ extern "C" int sgv_dequantize_rows(const void* q, int64_t q_stride, const float*
     if (!q || !scale || !out) return sgv_fail(SGV_ERR_INVALID_ARG, "dequantize_rows: NULL pointer");
     hipStream_t stream = (hipStream_t)stream_;
     sgv_launch_scope scope(SGV_K_RMS_NORM, stream, (double)rows * cols * (1.0 + sgv_dtype_size(dtype)));
-    // two vectors to a thread, up to a workgroup ([262144, 128] to bf16: 8 threads to a row 16 us, one 44, 64 52; [1000000, 5] to fp32: one thread 8.8 us, 64 138)
+    // two vectors to a thread, up to a workgroup ([262144, 128] to bf16: 8 threads to a row 16 us, one 44, 64 52; [1000000, 5] to fp32: one thread 8.6 us, 64 138)
     const int vec = dtype == SGV_F32 ? 4 : 8;
     int team = 1;
     while (team < 256 && 2 * team * vec < cols) team *= 2;
-    // (a call that mostly writes gains from 128 MB: [8192, 8192] to fp32 5.3 -> 6.7 TB/s)
+    // (a call that mostly writes gains from 128 MB: [8192, 8192] to fp32 5.4 -> 6.8 TB/s)
     const int past = sgv_rn::streams(3.0 * rows * cols * sgv_dtype_size(dtype), dtype, cols, {{out, cols}});
     const dim3 grid((unsigned)std::min<int64_t>((rows * team + 255) / 256, 1 << 16));
     const int8_t* in = (const int8_t*)q;

@@ -15,7 +15,7 @@ template <typename T, bool STREAM, bool DW, int WK, int TEAM, int NV>
 __global__ __launch_bounds__(TEAM <= 64 ? 256 : TEAM) void rms_norm_backward_kernel(const bwd_args p) {
     constexpr int VEC = io<T>::VEC, RPB = TEAM <= 64 ? 256 / TEAM : 1;
     constexpr bool TAIL = TEAM == 1;
-    // (1024 threads have 128 registers each: [8192, 9000] fp16 without the weight's gradient 88 -> 77 us with rows in flight, [4096, 10240] fp32 85 -> 109: spilled)
+    // (1024 threads have 128 registers each: [8192, 9000] fp16 without the weight's gradient 87 -> 74 us with rows in flight, [4096, 10240] fp32 84 -> 111: spilled)
     constexpr bool AHEAD = TEAM < 1024 || (!DW && VEC == 8);
     const bool partial = p.cols % VEC != 0;
     __shared__ red_slots red;

@@ -11,9 +11,9 @@
 // workgroups walk over rows with the next row's loads in flight while one is reduced and written, and hold the weight in registers.  Rows beyond 16384 elements are walked
 // over three times (the later reads come from the L2).  16-byte accesses need no alignment on this chip, so odd lengths and strides take the same kernels: a row's last,
 // partial vector is moved back to end with the row.  Calls that move more than the caches hold go past them.
-// Measured (a 1 GB copy: 5.2 TB/s): [16384, 4096] bf16 forward 42 us = 6.4 TB/s, with a residual 93 us = 5.8, to 8 bits 39 us = 5.2 (half of it instructions: 16 an
-// element), with a residual 76 us = 6.2, backward with all gradients 90 us = 5.9; [30000, 1111] fp16 forward 23 us = 5.7, backward with all gradients 74 us = 3.6 (rows off
-// the cache lines, eleven of 128 threads with a second vector).
+// Measured with a weight (a 1 GB copy: 5.2 TB/s): [16384, 4096] bf16 forward 41 us = 6.5 TB/s, with a residual 92 us = 5.9, to 8 bits 39 us = 5.2 (half of it instructions:
+// 16 an element), with a residual 75 us = 6.3, backward with all gradients 89 us = 6.0; [30000, 1111] fp16 forward 27 us = 5.0, backward with all gradients 73 us = 3.6 (few
+// waves in flight: the workgroups are held down by the partial sums below, and eleven of 128 threads have a second vector).
 //
 // Statistics are fp32: a lane sums at most 16 squares before the tree (fp64 in the walking kernels).  A row whose squares leave fp32's range (|h| > 1e18, or tiny rows under a
 // tiny eps) is summed again in fp64.  The 8-bit values are the correctly rounded ones: fp32 places a value to 5.4e-5 of a step, so a value within 6e-5 of a border
@@ -300,8 +300,10 @@ struct held_weight {
 };
 
 // How a row is held: TEAM threads with at most 16 elements each, or not at all (elems = 0, the walking kernels: 1024 threads for rows beyond 16384 elements).  Rows of
-// up to 64 vectors have as many lanes as vectors, up to a power of two ([262144, 128] bf16: a wave to a row 34 us forward, 53 to 8 bits, 102 backward with the weight's
-// gradient; 16 lanes 20.5, 20 and 41), rows shorter than a vector one ([1000000, 5] bf16: a wave 593 us forward, 5.0 ms backward; a thread 11 and 21 us).
+// up to 64 vectors have as many lanes as vectors, up to a power of two ([262144, 128] bf16: a wave to a row 34 us forward, 56 to 8 bits, 100 backward with the weight's
+// gradient; 16 lanes 20, 20 and 40), rows shorter than a vector one ([1000000, 5] bf16: a wave 593 us forward, 5.0 ms backward as it was first built; a thread 10 and 21 us).
+// 16 elements are what leaves registers for the next row's loads, the weight and its gradient's sums; rows beyond 16384 elements are walked over for it (forward 3.7 TB/s,
+// 1.4 to 1.5 to 8 bits or with the weight's gradient: [2048, 32768] bf16).
 struct shape { int team, elems; };
 static inline shape row_shape(int cols, int vec) {
     static const shape held[] = {{8, 4}, {16, 4}, {32, 4}, {64, 4}, {8, 8}, {16, 8}, {32, 8}, {64, 8}, {64, 16}, {128, 16}, {256, 16}, {512, 16}, {1024, 16}};
@@ -312,10 +314,10 @@ static inline shape row_shape(int cols, int vec) {
 constexpr int MAX_COLS = (1 << 26) - 1;
 
 // Workgroups of a launch, which walk over the rows: twice as many as 2048 threads to a CU, where rows are short; as many as the registers let a CU hold, 1024 threads, where
-// a row takes 512 threads or more ([4096, 16384] bf16 forward 41.5 us, four times as many 43.7; to 8 bits with a weight 44.4 and 49.5).  With a weight gradient they are the
-// rows of its partial sums, which should stay small beside the rows: one to a CU where a row takes 256 threads or more ([16384, 4096] bf16 with all gradients 89 us, two 94, four 108;
-// [4096, 16384] 102, 110, 124), four to a CU of 128 threads ([30000, 1111] fp16: 74 us, two 84, one 113), two of four short rows ([65536, 512] bf16: 52 us, one 62,
-// four 57); four rows to each at least ([2049, 1111] fp16: 13.4 us with two).
+// a row takes 512 threads or more ([4096, 16384] bf16 forward 40.8 us, four times as many 43.1; to 8 bits with a weight 44.6 and 49.5).  With a weight gradient they are the
+// rows of its partial sums, which should stay small beside the rows: one to a CU where a row takes 256 threads or more ([16384, 4096] bf16 with all gradients 89 us, two 92, four 107;
+// [4096, 16384] with the weight's 80, 89, 104), four to a CU of 128 threads ([30000, 1111] fp16: 59 us, two 74, one 104), two of four short rows ([65536, 512] bf16: 40 us, one
+// 57, four 43); four rows to each at least ([2049, 1111] fp16: 10.5 us, one workgroup to a CU 12.8, two rows to each 10.6).
 static inline int64_t groups(int64_t rows, const shape& s, bool dw) {
     const int threads = std::max(s.team, 256 * (s.team <= 64)), rpb = threads / s.team;
     const int64_t teams = (rows + rpb - 1) / rpb;
@@ -340,7 +342,8 @@ static void for_shape(const shape& s, F f) {
     else f.template go<1024, 16 / VEC>();
 }
 
-// Past the caches: calls that move more than 1.5 times the 256 MB Infinity Cache, over rows of whole aligned vectors.
+// Past the caches: calls that move more than 1.5 times the 256 MB Infinity Cache, over rows of whole aligned vectors ([16384, 4096] bf16 with a residual forward 98 -> 92 us,
+// backward 97 -> 89; the forward alone, 268 MB, would go from 41 to 44).
 struct rows_at { const void* p; int64_t stride; };
 static bool streams(double bytes, int dtype, int cols, std::initializer_list<rows_at> all) {
     const int64_t es = (int64_t)sgv_dtype_size(dtype);

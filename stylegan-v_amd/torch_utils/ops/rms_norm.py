@@ -13,7 +13,8 @@ transforms (``torch.func``) and while a graph of torch's operations is recorded 
 ``rms_norm_int8`` gives y in 8 bits with one scale per row -- the left operand of ``ops.int8.matmul`` -- in the same single pass: y is never written in its own type.
 It serves inference and has no gradient.
 
-Statistics are fp32 whatever the rows' type (fp32, fp16, bf16).  CPU tensors take the plain torch formulation.
+Statistics are fp32 whatever the rows' type (fp32, fp16, bf16), fp64 for rows whose squares leave fp32's range; eps and 1 / rms are fp32 numbers.  CPU tensors take the plain
+torch formulation.
 """
 import torch
 import torch.autograd.forward_ad as _fwd
@@ -94,7 +95,7 @@ def quantize_ref(u, factor):
 
 def rms_norm_int8(x, weight=None, residual=None, eps=1e-8):
     """``rms_norm`` with y in 8 bits: (q [..., K] int8, scale [...] fp32), with a residual (q, scale, h).  y stands for q * scale: scale = max|y| / 127 of each row and
-    q = y / scale rounded to nearest even (of the exact quotient).  A row of zeros has scale 0; a row with a NaN or an infinity in y has scale NaN and q = 0.
+    q = y / scale rounded to nearest even (of the exact quotient).  A row of zeros has scale 0 (NaN under eps = 0, as its y); a row with a NaN or an infinity in y has scale NaN and q = 0.
     The rows of q start on 16 bytes (q is a view of wider storage where K is no multiple of 16), as ``ops.int8.matmul`` wants them."""
     if isinstance(x, torch.Tensor) and x.is_cuda:
         out = launch_int8('rms_norm_int8', x, weight, residual, eps, True)
